@@ -12,7 +12,7 @@
  *     throws; infmoe_last_error() gives a thread-local message;
  *   - pointers named d_* are device pointers on the current CUDA device,
  *     h_* are host pointers; `stream` is a cudaStream_t passed as void*;
- *   - all tensors are FP32, row-major, indices are int32;
+ *   - all tensors are FP32 (unless a dtype argument says otherwise), row-major, indices are int32;
  *   - work is ordered on `stream`; unless a function says so it does not
  *     block the host.
  */
@@ -146,6 +146,16 @@ INFMOE_API int infmoe_layer_expert_forward_scatter(infmoe_layer* layer, const fl
                                                    const int32_t* d_expert_of_row, const float* d_row_score,
                                                    const uint64_t* d_row_dst, void* d_workspace,
                                                    size_t workspace_bytes, int64_t rows, void* stream);
+
+/* A pass in which every token goes to several experts: out[t] = x[t] + sum_s weight[t][s] * (E_s(x[t]) - x[t]) with E_s the
+ * expert gate[t][s] (T5_FF: E(x) = x + f(x), so x[t] + sum_s weight[t][s] * f_s(x[t])).  d_gate [token_num][top_k] and
+ * d_weight [token_num][top_k] come from infmoe_expert_select_topk; a gate outside [0, expert_count) is a place without an
+ * expert, and a token without any passes unchanged.  Experts resident, streamed or of a registered sublayer as in
+ * infmoe_layer_enqueue; the variant's own routing and output mix play no part.  No counterpart in the reference (top-1). */
+INFMOE_API int infmoe_layer_topk_workspace_bytes(const infmoe_layer* layer, int64_t token_num, int32_t top_k, size_t* bytes);
+INFMOE_API int infmoe_layer_forward_topk(infmoe_layer* layer, const float* d_input, const int32_t* d_gate,
+                                         const float* d_weight, int64_t token_num, int32_t top_k, float* d_output,
+                                         void* d_workspace, size_t workspace_bytes, void* stream);
 
 /* Blocks until `stream` is idle and returns the device-side status of the calls enqueued so far. */
 INFMOE_API int infmoe_layer_sync_status(infmoe_layer* layer, void* stream);
@@ -396,6 +406,86 @@ INFMOE_API int infmoe_t5ff_static_limit(int64_t rows, int32_t embedding_size, in
 INFMOE_API int infmoe_t5ff_run_static(int64_t rows, int32_t embedding_size, int32_t hidden_size,
                                       const float* d_ln_w, const float* d_wi0, const float* d_wi1,
                                       const float* d_wo, const float* d_x, float* d_y, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Several experts per token, and adapters of requests                        */
+/* ------------------------------------------------------------------------ */
+/* No counterparts in the reference (top-k routing is a TODO there).  Unlike the
+ * functions above these take FP32, FP16 or BF16 elements; all of them compute in
+ * FP32 or more and round once, when they store. */
+typedef enum infmoe_dtype { INFMOE_F32 = 0, INFMOE_F16 = 1, INFMOE_BF16 = 2 } infmoe_dtype;
+typedef enum infmoe_score { INFMOE_SCORE_SOFTMAX = 0, INFMOE_SCORE_SIGMOID = 1 } infmoe_score;
+
+typedef struct infmoe_topk_config {
+    int32_t expert_count;
+    int32_t top_k;                     /* experts of a token, 1..32 */
+    int32_t score;                     /* infmoe_score of a row's logits */
+    int32_t group_count;               /* 1: no groups; else a divisor of expert_count, at most 32: experts in equal groups */
+    int32_t top_groups;                /* groups a token chooses from, 1..group_count */
+    int32_t group_best;                /* a group counts with its best expert (1) or with the sum of its two best (2) */
+    int32_t renormalise;               /* != 0: the weights of a token's experts sum to `scale` */
+    float scale;                       /* factor of all weights */
+} infmoe_topk_config;
+
+/* The top_k best experts of every token, best first, and their weights.  d_logits [token_num][ld] (row stride ld in
+ * elements, >= expert_count): gating logits.  Scores s are the softmax of a row or the sigmoid of each logit; experts and
+ * groups are chosen by s + d_bias[e] (d_bias [expert_count] or NULL: none), weights are s alone, so a bias balances the load
+ * without showing in the result.  The choice is that of these sums in 64 bits (without a bias experts stand in the order of
+ * their logits, and so do groups that count with one expert); ties go to the lowest index.
+ * An expert whose logit is NaN or the type's lowest value or less (-inf included) is never chosen and is no part of the
+ * softmax; one whose bias is NaN or -inf is never chosen.  Where fewer than top_k experts are left, the remaining places get
+ * gate -1 and weight 0; a token with none at all also sets bit 0 of d_status (may be NULL), like infmoe_expert_select.
+ * d_gate, d_weight: [token_num][top_k].  At most 32 groups, and 32 experts to each of the 32 / (groups rounded up to a power
+ * of two) lanes that work on a group (1024 experts without groups). */
+INFMOE_API int infmoe_expert_select_topk(const infmoe_topk_config* cfg, int64_t token_num, const void* d_logits,
+                                         int32_t dtype, int64_t ld, const float* d_bias, int32_t* d_gate, float* d_weight,
+                                         int32_t* d_status, void* stream);
+
+/* Token rows in expert order, once per chosen expert.  A slot is a place of gate[token_num][top_k]; d_pos [token_num *
+ * top_k] and the row count *d_valid_rows are what infmoe_expert_count makes of gate seen as token_num * top_k gates (d_pos,
+ * and d_offset + expert_count).  routed[j] = input[pos[j] / top_k] for the rows j < *d_valid_rows; the other rows of
+ * d_routed are left as they were.  d_row_of (may be NULL) [token_num][top_k]: the row of every slot, -1 for a slot without
+ * an expert. */
+INFMOE_API int infmoe_expert_scatter_topk(int64_t token_num, int32_t top_k, int32_t token_len, int32_t dtype,
+                                          const void* d_input, int64_t ld, const int32_t* d_pos, const int32_t* d_valid_rows,
+                                          void* d_routed, int32_t* d_row_of, void* stream);
+
+/* The experts' results of every token put together: out[t] = sum_s weight[t][s] * rows[row_of[t][s]], slots in ascending
+ * order.  d_row_of NULL: slot (t, s) is row t * top_k + s.  d_gate (may be NULL): slots with a negative gate are left out,
+ * and so are slots whose row lies outside [0, rows).  With d_residual [token_num][token_len] the token's own row fills what
+ * the weights leave of one, out[t] += (1 - sum_s weight[t][s]) * residual[t], which is infmoe_expert_mix_gather's mix for
+ * several experts; for results that hold the row already (T5_FF: y = x + f(x)) it amounts to x + sum_s weight * f_s(x).
+ * d_output [token_num][token_len] may be d_residual, not d_rows. */
+INFMOE_API int infmoe_expert_combine_topk(int64_t token_num, int32_t top_k, int32_t token_len, int32_t dtype,
+                                          const void* d_rows, int64_t rows, const float* d_weight, const int32_t* d_gate,
+                                          const int32_t* d_row_of, const void* d_residual, void* d_output, void* stream);
+
+/* Low-rank adapters beside a projection that all requests share: out[t] = y[t] + scale[a] * B[a] (A[a] x[t]) for the
+ * tokens t of adapter a; out[t] = y[t] for tokens without one. */
+#define INFMOE_ADAPTER_MAX_RANK 128
+typedef struct infmoe_adapter_set {
+    int32_t adapter_count;
+    int32_t rank;                      /* rows of A and columns of B, 1..INFMOE_ADAPTER_MAX_RANK */
+    int32_t d_in, d_out;               /* widths of x and y */
+    int32_t dtype;                     /* infmoe_dtype of A, B, x, y and out */
+    const void* d_a;                   /* [adapter_count][rank][d_in] */
+    const void* d_b;                   /* [adapter_count][d_out][rank] */
+    const float* d_scale;              /* [adapter_count], or NULL: 1 */
+    const int32_t* d_rank;             /* [adapter_count], or NULL: all `rank`.  Only the first d_rank[a] rows of A[a] and
+                                          columns of B[a] count (values outside 0..rank are brought into it) */
+} infmoe_adapter_set;
+
+/* What a batch's tokens need for any number of infmoe_adapter_apply calls: the tokens grouped by adapter (in token order
+ * inside each, with the kernel of infmoe_expert_count) and cut into tiles.  d_adapter_of_token [token_num]; an index outside
+ * [0, adapter_count) means none.  d_plan: infmoe_adapter_plan_bytes, 16-byte aligned.  Holds for adapter sets of
+ * adapter_count adapters and batches of token_num tokens. */
+INFMOE_API int infmoe_adapter_plan_bytes(int64_t token_num, int32_t adapter_count, size_t* bytes);
+INFMOE_API int infmoe_adapter_plan(int64_t token_num, int32_t adapter_count, const int32_t* d_adapter_of_token, void* d_plan,
+                                   size_t plan_bytes, void* stream);
+/* d_x [token_num][ldx], d_y [token_num][ldy], d_out [token_num][ldo], strides in elements.  d_out may be d_y (rows of
+ * tokens without an adapter are then not touched), not d_x.  No workspace. */
+INFMOE_API int infmoe_adapter_apply(const infmoe_adapter_set* set, int64_t token_num, const void* d_x, int64_t ldx,
+                                    const void* d_y, int64_t ldy, void* d_out, int64_t ldo, const void* d_plan, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,90 @@
+"""Low-rank adapters of many requests at once, beside a projection they share (torch tensors over the C ABI).
+
+    adapters = Adapters(a, b, scale)                 # a [n, r, d_in], b [n, d_out, r]
+    plan = adapters.plan(adapter_of_token)           # once per batch: int32 [T], -1 = none
+    out = adapters.apply(x, y, plan)                 # y + scale * b (a x), row by row with the row's adapter
+
+A plan holds for every projection of the batch whose set has as many adapters.  `MoELayer.forward(x, adapters=..., plan=...)`
+adds the adapters of a layer's requests to its output.
+"""
+from __future__ import annotations
+
+import ctypes
+
+from . import capi
+from .topk import check_array, dtype_code, launch, rows_of
+
+__all__ = ["Adapters", "AdapterPlan"]
+
+
+class AdapterPlan:
+    """A batch's tokens grouped by adapter (infmoe_adapter_plan)."""
+
+    def __init__(self, adapter_of_token, adapter_count: int) -> None:
+        import torch
+
+        if not adapter_of_token.is_cuda or adapter_of_token.dtype != torch.int32 or not adapter_of_token.is_contiguous():
+            raise ValueError("adapter_of_token must be a contiguous int32 CUDA tensor")
+        self.tokens, self.adapter_count, self.device = adapter_of_token.numel(), int(adapter_count), adapter_of_token.device
+        need = ctypes.c_size_t()
+        capi.check(capi.lib().infmoe_adapter_plan_bytes(self.tokens, self.adapter_count, ctypes.byref(need)))
+        self.buffer = torch.empty(need.value, dtype=torch.uint8, device=self.device)
+        launch(adapter_of_token.get_device(), "infmoe_adapter_plan", self.tokens, self.adapter_count,
+               adapter_of_token.data_ptr(), self.buffer.data_ptr(), need.value)
+
+
+class Adapters:
+    """A set of low-rank adapters of one projection (infmoe_adapter_set).
+
+    a [n, r, d_in] and b [n, d_out, r]: contiguous CUDA tensors, float32, float16 or bfloat16 (the type of x and y too); they
+    are used in place, not copied.  scale: a number, or a float32 tensor [n].  rank: int32 tensor [n], of which adapter i uses
+    only the first rank[i] rows of a[i] and columns of b[i]; None: all r."""
+
+    def __init__(self, a, b, scale=1.0, rank=None) -> None:
+        import torch
+
+        if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2] or a.dtype != b.dtype or \
+                a.device != b.device or not a.is_cuda or not a.is_contiguous() or not b.is_contiguous():
+            raise ValueError("a [n, r, d_in] and b [n, d_out, r] must be contiguous CUDA tensors of one type and device")
+        n, r, d_in = a.shape
+        self.dtype, self.device = a.dtype, a.device
+        self.adapter_count, self.rank, self.d_in, self.d_out = n, r, d_in, b.shape[1]
+        if isinstance(scale, (int, float)):
+            scale = None if scale == 1 else torch.full((n,), float(scale), dtype=torch.float32, device=a.device)
+        if scale is not None:
+            check_array(scale, (n,), torch.float32, a.device, "scale")
+        if rank is not None:
+            check_array(rank, (n,), torch.int32, a.device, "rank")
+        self._tensors = (a, b, scale, rank)
+        self._set = capi.AdapterSet(n, r, d_in, self.d_out, dtype_code(a), a.data_ptr(), b.data_ptr(),
+                                    scale.data_ptr() if scale is not None else None,
+                                    rank.data_ptr() if rank is not None else None)
+        self._set_ref = ctypes.byref(self._set)
+        # what a set can be refused for, now and not at the first call: no tokens, no device work
+        capi.check(capi.lib().infmoe_adapter_apply(self._set_ref, 0, None, d_in, None, self.d_out, None, self.d_out, None, None))
+
+    def plan(self, adapter_of_token) -> AdapterPlan:
+        """adapter_of_token: int32 CUDA tensor, one index per token; an index outside [0, n) means none."""
+        return AdapterPlan(adapter_of_token, self.adapter_count)
+
+    def apply(self, x, y, plan: AdapterPlan, out=None):
+        """x [..., d_in], y [..., d_out] -> y plus each row's adapter of x.  out may be y (in place), not x."""
+        import torch
+
+        T, ldx = rows_of(x, self.d_in, "x")
+        Ty, ldy = rows_of(y, self.d_out, "y")
+        if x.dtype != self.dtype or y.dtype != self.dtype or x.device != self.device or y.device != self.device:
+            raise ValueError(f"x and y must be {str(self.dtype)[6:]} tensors on {self.device}, like the adapters")
+        if T != Ty or T != plan.tokens or plan.adapter_count != self.adapter_count or plan.device != self.device:
+            raise ValueError(f"x has {T} rows, y {Ty}; the plan is for {plan.tokens} rows and {plan.adapter_count} adapters on "
+                             f"{plan.device}, the set has {self.adapter_count} on {self.device}")
+        if out is None:
+            out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+            ldo = self.d_out
+        else:
+            To, ldo = rows_of(out, self.d_out, "out")
+            if To != T or out.shape != y.shape or out.dtype != self.dtype or out.device != self.device:
+                raise ValueError("out must be a tensor like y")
+        launch(x.get_device(), "infmoe_adapter_apply", self._set_ref, T, x.data_ptr(), ldx, y.data_ptr(), ldy, out.data_ptr(),
+               ldo, plan.buffer.data_ptr())
+        return out

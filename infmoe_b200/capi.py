@@ -65,6 +65,41 @@ class EpConfig(ctypes.Structure):
     ]
 
 
+class TopKConfig(ctypes.Structure):
+    """struct infmoe_topk_config"""
+
+    _fields_ = [
+        ("expert_count", ctypes.c_int32),
+        ("top_k", ctypes.c_int32),
+        ("score", ctypes.c_int32),
+        ("group_count", ctypes.c_int32),
+        ("top_groups", ctypes.c_int32),
+        ("group_best", ctypes.c_int32),
+        ("renormalise", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
+class AdapterSet(ctypes.Structure):
+    """struct infmoe_adapter_set"""
+
+    _fields_ = [
+        ("adapter_count", ctypes.c_int32),
+        ("rank", ctypes.c_int32),
+        ("d_in", ctypes.c_int32),
+        ("d_out", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("d_a", ctypes.c_void_p),
+        ("d_b", ctypes.c_void_p),
+        ("d_scale", ctypes.c_void_p),
+        ("d_rank", ctypes.c_void_p),
+    ]
+
+
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2      # infmoe_dtype
+SCORES = {"softmax": 0, "sigmoid": 1}           # infmoe_score
+ADAPTER_MAX_RANK = 128
+
 EP_ID_BYTES = 128
 
 SUB_INIT_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_char_p)
@@ -109,6 +144,8 @@ SIGNATURES = {
     "infmoe_layer_enqueue": [_vp, _vp, _vp, _vp, _sz, _i64, _vp],
     "infmoe_layer_expert_forward": [_vp, _vp, _vp, _vp, _vp, _sz, _i64, _vp],
     "infmoe_layer_expert_forward_scatter": [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _vp],
+    "infmoe_layer_topk_workspace_bytes": [_vp, _i64, _i32, ctypes.POINTER(_sz)],
+    "infmoe_layer_forward_topk": [_vp, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _sz, _vp],
     "infmoe_layer_sync_status": [_vp, _vp],
     "infmoe_layer_forward_host": [_vp, _vp, _vp, _i64],
     "infmoe_layer_submit_host": [_vp, _vp, _vp, _i64],
@@ -135,6 +172,12 @@ SIGNATURES = {
     "infmoe_t5ff_run": [_i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp],
     "infmoe_t5ff_static_limit": [_i64, _i32, _i32, ctypes.POINTER(_sz), ctypes.POINTER(_sz)],
     "infmoe_t5ff_run_static": [_i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "infmoe_expert_select_topk": [ctypes.POINTER(TopKConfig), _i64, _vp, _i32, _i64, _vp, _vp, _vp, _vp, _vp],
+    "infmoe_expert_scatter_topk": [_i64, _i32, _i32, _i32, _vp, _i64, _vp, _vp, _vp, _vp, _vp],
+    "infmoe_expert_combine_topk": [_i64, _i32, _i32, _i32, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp],
+    "infmoe_adapter_plan_bytes": [_i64, _i32, ctypes.POINTER(_sz)],
+    "infmoe_adapter_plan": [_i64, _i32, _vp, _vp, _sz, _vp],
+    "infmoe_adapter_apply": [ctypes.POINTER(AdapterSet), _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp],
     "infmoe_register_sublayer": [ctypes.c_char_p, ctypes.POINTER(SublayerVtable)],
     "infmoe_ep_unique_id": [_vp],
     "infmoe_ep_create": [ctypes.POINTER(EpConfig), ctypes.POINTER(_vp)],

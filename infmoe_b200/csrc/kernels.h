@@ -1,4 +1,4 @@
-// Launchers of the CUDA kernels (defined in route.cu, dispatch.cu, rows.cu, ffn_simt.cu, ffn_umma.cu).
+// Launchers of the CUDA kernels (defined in route.cu, dispatch.cu, rows.cu, ffn_simt.cu, ffn_umma.cu, topk.cu).
 #pragma once
 
 #include <cuda.h>
@@ -112,5 +112,14 @@ constexpr int FFN_COUNTERS = FFN_CTAS * 16;      // ints in part_count: one per 
 size_t ffn_umma_part_bytes(long long T, int D, int F);
 // Rows of `in` [n][D] copied to the addresses dst[i] (one per row; they may point into a peer GPU's memory).
 int launch_rows_to_ptrs(long long n, int D, const float* in, const unsigned long long* dst, cudaStream_t stream);
+
+
+// Rows to k experts and back (arguments checked by infmoe_expert_scatter_topk / infmoe_expert_combine_topk).  pos NULL: row j
+// is slot j; valid_rows NULL: all rows.  A slot whose gate lies outside [0, gates) has no row (gate NULL: all have one).
+int launch_scatter_topk(long long rows, int k, int D, int elem_bytes, const void* x, long long ldx, const int* pos,
+                        const int* valid_rows, void* routed, int* row_of, cudaStream_t stream);
+int launch_combine_topk(long long tokens, int k, int D, int dtype, const void* y, long long rows, const float* weight,
+                        const int* gate, unsigned gates, const int* row_of, const void* x, void* out,
+                        cudaStream_t stream);
 
 }  // namespace infmoe

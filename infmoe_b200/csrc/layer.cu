@@ -1019,10 +1019,11 @@ int infmoe_layer_workspace_bytes(const infmoe_layer* L, int64_t T, size_t* bytes
 // routing happened on the rank that owns the token.
 // region_count / region_size (expert-parallel receive buffer): the T rows are slots in regions of region_size, of
 // which only the first region_count[s] of region s hold a row.
+// some_without: a gate outside [0, E) is a row without an expert and no error.
 static int layer_run(infmoe_layer* L, const float* d_in, float* d_out, void* d_ws, size_t ws_bytes, int64_t T,
                      void* stream_v, const int* given_gate, const float* row_score = nullptr,
                      const unsigned long long* row_dst = nullptr, const int* region_count = nullptr,
-                     int region_size = 0) {
+                     int region_size = 0, bool some_without = false) {
     if (!L || T < 0 || (T > 0 && (!d_in || (!d_out && !row_dst) || !d_ws))) {
         set_error("layer_enqueue: bad argument");
         return INFMOE_ERR_INVALID_ARGUMENT;
@@ -1104,8 +1105,9 @@ static int layer_run(infmoe_layer* L, const float* d_in, float* d_out, void* d_w
     const bool with_scatter = !L->identity && !L->custom && !region_count && dispatch_supported(L->E) &&
                               dispatch_scatter_supported(T, L->D, L->E, d_in, pack);
     int* const zero = w.part_bytes ? buf.part_count : nullptr;
+    int* const gate_status = some_without ? nullptr : L->d_status;
     if (!with_scatter)
-        INFMOE_TRY(launch_dispatch(gate_in, T, L->E, pos, count, offset, L->d_status, stream, region_count, region_size,
+        INFMOE_TRY(launch_dispatch(gate_in, T, L->E, pos, count, offset, gate_status, stream, region_count, region_size,
                                    zero, FFN_COUNTERS));
     const int* valid_rows = offset + L->E;   // rows past it have no expert (or are empty slots): nobody touches them
     INFMOE_TRY(prof_mark(L, 2, stream));
@@ -1184,7 +1186,7 @@ static int layer_run(infmoe_layer* L, const float* d_in, float* d_out, void* d_w
         }
         if (with_scatter) {
             INFMOE_TRY(launch_dispatch_scatter(T, L->D, L->E, d_in, score, gate_in, gamma, gamma_stride, pos, count, offset,
-                                               L->d_status, zero, FFN_COUNTERS, rscore, buf.h, buf.row_info, pack,
+                                               gate_status, zero, FFN_COUNTERS, rscore, buf.h, buf.row_info, pack,
                                                !given_gate, stream));
         } else if (pack) {
             INFMOE_TRY(launch_scatter_ln_pack(0, T, L->D, d_in, score, pos, gate_in, gamma, gamma_stride, valid_rows,
@@ -1330,6 +1332,57 @@ int infmoe_layer_expert_forward(infmoe_layer* L, const float* d_rows, const int3
     }
     if (rows == 0) return INFMOE_OK;
     return layer_run(L, d_rows, d_out, d_ws, ws_bytes, rows, stream_v, d_expert_of_row);
+}
+
+// The rows of a top-k pass: the layer's own workspace for T * k rows, the tokens' rows k times, and the experts' results.
+static int topk_workspace(const char* what, const infmoe_layer* L, int64_t T, int32_t k, size_t* layer_bytes, size_t* row_bytes) {
+    if (!L || T < 0 || k <= 0) {
+        set_error("%s: bad argument (T=%lld top_k=%d)", what, (long long)T, k);
+        return INFMOE_ERR_INVALID_ARGUMENT;
+    }
+    if (T > 0x7fffffffLL / k / (L->D > L->F ? L->D : L->F)) {
+        set_error("%s: %lld tokens of %d experts are too many for 32-bit row offsets", what, (long long)T, k);
+        return INFMOE_ERR_UNSUPPORTED;
+    }
+    INFMOE_TRY(infmoe_layer_workspace_bytes(L, T * k, layer_bytes));
+    *layer_bytes = align_up(*layer_bytes);
+    *row_bytes = align_up(sizeof(float) * (size_t)T * (size_t)k * (size_t)L->D);
+    return INFMOE_OK;
+}
+
+int infmoe_layer_topk_workspace_bytes(const infmoe_layer* L, int64_t T, int32_t k, size_t* bytes) {
+    size_t layer_bytes, row_bytes;
+    INFMOE_TRY(topk_workspace("layer_topk_workspace_bytes", L, T, k, &layer_bytes, &row_bytes));
+    if (!bytes) {
+        set_error("layer_topk_workspace_bytes: bad argument");
+        return INFMOE_ERR_INVALID_ARGUMENT;
+    }
+    *bytes = layer_bytes + 2 * row_bytes + ALIGN;
+    return INFMOE_OK;
+}
+
+int infmoe_layer_forward_topk(infmoe_layer* L, const float* d_in, const int32_t* d_gate, const float* d_weight, int64_t T,
+                              int32_t k, float* d_out, void* d_ws, size_t ws_bytes, void* stream_v) {
+    size_t layer_bytes, row_bytes;
+    INFMOE_TRY(topk_workspace("layer_forward_topk", L, T, k, &layer_bytes, &row_bytes));
+    if (T == 0) return INFMOE_OK;
+    if (!d_in || !d_gate || !d_weight || !d_out || !d_ws || d_in == d_out) {
+        set_error("layer_forward_topk: bad argument (input and output must not alias)");
+        return INFMOE_ERR_INVALID_ARGUMENT;
+    }
+    if (ws_bytes < layer_bytes + 2 * row_bytes + ALIGN) {
+        set_error("layer_forward_topk: workspace of %zu bytes is too small, %zu needed", ws_bytes,
+                  layer_bytes + 2 * row_bytes + ALIGN);
+        return INFMOE_ERR_INVALID_ARGUMENT;
+    }
+    cudaStream_t stream = (cudaStream_t)stream_v;
+    char* base = (char*)(((uintptr_t)d_ws + ALIGN - 1) / ALIGN * ALIGN);
+    float* rows = (float*)(base + layer_bytes);
+    float* results = (float*)(base + layer_bytes + row_bytes);
+    INFMOE_TRY(launch_scatter_topk(T * k, k, L->D, (int)sizeof(float), d_in, L->D, nullptr, nullptr, rows, nullptr, stream));
+    INFMOE_TRY(layer_run(L, rows, results, base, layer_bytes, T * k, stream_v, d_gate, nullptr, nullptr, nullptr, 0, true));
+    return launch_combine_topk(T, k, L->D, INFMOE_F32, results, T * k, d_weight, d_gate, (unsigned)L->E, nullptr, d_in, d_out,
+                               stream);
 }
 
 int infmoe_layer_expert_forward_scatter(infmoe_layer* L, const float* d_rows, const int32_t* d_expert_of_row,

@@ -1,0 +1,420 @@
+// Routing to the k best experts, and token rows to k experts and back.  The reference routes to one expert (top-k is a TODO
+// there); these kernels stand beside its select / scatter / gather (plugin/cuda/moe.cu:147-258) for layers that route to k.
+#include <cfloat>
+#include <type_traits>
+
+#include "common.cuh"
+#include "elem.cuh"
+#include "kernels.h"
+
+namespace infmoe {
+
+namespace {
+
+constexpr int SELECT_WARPS = 8;
+
+// Experts are laid out over the lanes of a warp so that a group's experts sit on lanes of their own: groups are padded to a
+// power of two, group g has `lanes` = 32 / padded lanes, and each of these holds V consecutive experts of the group.  So
+// lane order, and place order inside a lane, is expert order, and the lowest lane and place win ties.
+struct SelectArgs {
+    const void* logits;      // [T][ld]
+    long long T, ld;
+    int E, k, groups, top_groups, group_best, group_size, lanes;
+    int sigmoid, renormalise;
+    float scale;
+    const float* bias;       // [E] or NULL
+    int* gate;               // [T][k]
+    float* weight;           // [T][k]
+    int* status;
+};
+
+template <typename T>
+struct Lowest;
+template <> struct Lowest<float> { static __device__ float value() { return -FLT_MAX; } };
+template <> struct Lowest<__half> { static __device__ float value() { return -65504.f; } };
+template <> struct Lowest<__nv_bfloat16> { static __device__ float value() { return __uint_as_float(0xff7f0000u); } };
+
+__device__ __forceinline__ double shfl_xor(double v, int off) { return __shfl_xor_sync(0xffffffffu, v, off); }
+
+// Expert indices of the k best in lanes 0..k-1, -1 where there are fewer, chosen by scores in 64 bits.
+template <typename T, int V>
+__device__ int select_in_64_bits(const SelectArgs& a, long long t, int lane) {
+    const T* row = static_cast<const T*>(a.logits) + t * a.ld;
+    const int g = lane / a.lanes, first = (lane - g * a.lanes) * V;
+    const double none = -INFINITY;
+    double c[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const bool in = g < a.groups && first + j < a.group_size;
+        const float l = in ? to_float(row[g * a.group_size + first + j]) : -INFINITY;
+        c[j] = l > Lowest<T>::value() ? (double)l : none;      // false for NaN too
+    }
+    // Without a bias the logits order the experts: scores would order them the same, but for those that round to one value.
+    double top = none, sum = 0.0;
+    if (!a.sigmoid && (a.bias || (a.groups > 1 && a.group_best == 2))) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) top = fmax(top, c[j]);
+        for (int off = 16; off >= 1; off >>= 1) top = fmax(top, shfl_xor(top, off));
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum += c[j] == none ? 0.0 : c[j] == top ? 1.0 : exp(c[j] - top);
+        for (int off = 16; off >= 1; off >>= 1) sum += shfl_xor(sum, off);
+    }
+    const auto score_of = [&](double l) {
+        return a.sigmoid ? 1.0 / (1.0 + exp(-l)) : (l == top ? 1.0 : exp(l - top)) / sum;
+    };
+    if (a.bias) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if (c[j] == none) continue;
+            const float b = a.bias[g * a.group_size + first + j];
+            c[j] = b > -INFINITY ? score_of(c[j]) + (double)b : none;
+        }
+    }
+    if (a.groups > 1) {
+        // the two best of the group, then the groups best first
+        double b1 = none, b2 = none;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            b2 = fmax(b2, fmin(b1, c[j]));
+            b1 = fmax(b1, c[j]);
+        }
+        for (int off = a.lanes >> 1; off >= 1; off >>= 1) {
+            const double o1 = shfl_xor(b1, off), o2 = shfl_xor(b2, off);
+            b2 = fmax(fmin(b1, o1), fmax(b2, o2));
+            b1 = fmax(b1, o1);
+        }
+        double score = b1;
+        if (a.group_best == 2 && b1 > none) {
+            score = a.bias ? b1 : score_of(b1);
+            if (b2 > none) score += a.bias ? b2 : score_of(b2);
+        }
+        int better = 0;
+        for (int o = 0; o < a.groups; ++o) {
+            const double other = __shfl_sync(0xffffffffu, score, o * a.lanes);
+            better += other > score || (other == score && o < g);
+        }
+        if (better >= a.top_groups)
+#pragma unroll
+            for (int j = 0; j < V; ++j) c[j] = none;
+    }
+    int mine = -1;
+    for (int i = 0; i < a.k; ++i) {
+        double best = none;
+#pragma unroll
+        for (int j = 0; j < V; ++j) best = fmax(best, c[j]);
+        double top = best;
+        for (int off = 16; off >= 1; off >>= 1) top = fmax(top, shfl_xor(top, off));
+        if (!(top > none)) break;
+        const int owner = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
+        int place = 0;
+#pragma unroll
+        for (int j = V - 1; j >= 0; --j) place = c[j] == top ? j : place;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (lane == owner && j == place) c[j] = none;
+        const int e = __shfl_sync(0xffffffffu, g * a.group_size + first + place, owner);
+        if (lane == i) mine = e;
+    }
+    return mine;
+}
+
+// Weights of the chosen experts, whose indices lanes 0..k-1 hold, and the row's answer.  Renormalised weights are computed
+// from the chosen logits alone, relative to the largest, so they do not vanish where all scores do.
+template <typename T, int V>
+__device__ void store_choice(const SelectArgs& a, long long t, int lane, int mine) {
+    const T* row = static_cast<const T*>(a.logits) + t * a.ld;
+    const float l = mine >= 0 ? to_float(row[mine]) : -INFINITY;
+    const float top = warp_max(l);
+    float w = 0.f;
+    if (a.renormalise) {
+        if (a.sigmoid && !(top > 0.f))
+            w = mine >= 0 ? expf(l - top) / (1.f + expf(l)) : 0.f;
+        else if (a.sigmoid)
+            w = mine >= 0 ? 1.f / (1.f + expf(-l)) : 0.f;
+        else
+            w = mine >= 0 ? (l == top ? 1.f : expf(l - top)) : 0.f;
+        const float sum = warp_xor_sum(w);
+        w = mine >= 0 ? w / sum : 0.f;
+    } else if (a.sigmoid) {
+        w = mine >= 0 ? 1.f / (1.f + expf(-l)) : 0.f;
+    } else {
+        // the sum over all experts of the row
+        float all = -INFINITY, sum = 0.f;
+        for (int e = lane; e < a.E; e += 32) {
+            const float v = to_float(row[e]);
+            all = v > Lowest<T>::value() ? fmaxf(all, v) : all;
+        }
+        all = warp_max(all);
+        for (int e = lane; e < a.E; e += 32) {
+            const float v = to_float(row[e]);
+            if (v > Lowest<T>::value()) sum += v == all ? 1.f : expf(v - all);
+        }
+        sum = warp_xor_sum(sum);
+        w = mine >= 0 ? (l == all ? 1.f : expf(l - all)) / sum : 0.f;
+    }
+    if (lane < a.k) {
+        a.gate[t * a.k + lane] = mine;
+        a.weight[t * a.k + lane] = w * a.scale;
+    }
+    if (lane == 0 && mine < 0 && a.status) atomicOr(a.status, STATUS_NO_EXPERT);
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(SELECT_WARPS * 32) select_topk_kernel(const SelectArgs a) {
+    pdl_trigger();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const long long t = (long long)blockIdx.x * SELECT_WARPS + (threadIdx.x >> 5);
+    if (t >= a.T) return;
+    const int mine = select_in_64_bits<T, V>(a, t, lane);
+    store_choice<T, V>(a, t, lane, mine);
+}
+
+template <typename T, int V>
+int launch_select(const SelectArgs& a, cudaStream_t stream) {
+    const long long grid = (a.T + SELECT_WARPS - 1) / SELECT_WARPS;
+    INFMOE_CUDA_TRY(launch_chained(select_topk_kernel<T, V>, (unsigned)grid, SELECT_WARPS * 32, 0, 1, stream, a));
+    note_launch();
+    INFMOE_CUDA_TRY(cudaGetLastError());
+    return INFMOE_OK;
+}
+
+template <typename T>
+int launch_select_type(const SelectArgs& a, int per_lane, cudaStream_t stream) {
+    if (per_lane <= 1) return launch_select<T, 1>(a, stream);
+    if (per_lane <= 2) return launch_select<T, 2>(a, stream);
+    if (per_lane <= 4) return launch_select<T, 4>(a, stream);
+    if (per_lane <= 8) return launch_select<T, 8>(a, stream);
+    if (per_lane <= 16) return launch_select<T, 16>(a, stream);
+    return launch_select<T, 32>(a, stream);
+}
+
+// ---- rows to k experts and back ------------------------------------------------------------------
+
+constexpr int ROW_THREADS = 256;
+
+// How a block of ROW_THREADS shares out rows of `vecs` vectors: rows_per_block whole rows, or (one row per block) parts of a
+// row along grid.y.
+struct RowSplit {
+    int vecs, rows_per_block;
+};
+
+// routed[j] = x[pos[j] / k] and row_of[pos[j]] = j for the rows j below *valid_rows; row_of = -1 for the slots of the others.
+// pos NULL: row j is slot j; valid_rows NULL: all rows.
+template <typename Vec>
+__global__ void __launch_bounds__(ROW_THREADS)
+scatter_topk_kernel(long long rows, int k, RowSplit split, const Vec* x, long long ldx, const int* pos, const int* valid_rows,
+                    Vec* __restrict__ routed, int* __restrict__ row_of) {
+    pdl_wait();
+    pdl_trigger();
+    int local = 0, v = (int)threadIdx.x + (int)blockIdx.y * ROW_THREADS;
+    if (split.rows_per_block > 1) {
+        local = v / split.vecs;
+        v -= local * split.vecs;
+    }
+    const long long j = (long long)blockIdx.x * split.rows_per_block + local;
+    if (local >= split.rows_per_block || v >= split.vecs || j >= rows) return;
+    const int p = pos ? pos[j] : (int)j;
+    if (p < 0 || p >= rows) return;
+    const bool valid = !valid_rows || j < *valid_rows;
+    if (v == 0 && row_of) row_of[p] = valid ? (int)j : -1;
+    if (valid) routed[j * split.vecs + v] = x[(long long)(p / k) * ldx + v];
+}
+
+// out[t] = sum_s w[t][s] y[row_of[t][s]] (+ (1 - sum_s w[t][s]) x[t]), slots without a row left out: a row outside [0, rows),
+// or a gate outside [0, gates).
+template <typename T, int N, bool RESIDUAL>
+__global__ void __launch_bounds__(ROW_THREADS)
+combine_topk_kernel(long long tokens, int k, RowSplit split, const T* y, long long rows, const float* weight, const int* gate,
+                    unsigned gates, const int* row_of, const T* x, T* __restrict__ out) {
+    pdl_trigger();
+    pdl_wait();
+    int local = 0, v = (int)threadIdx.x + (int)blockIdx.y * ROW_THREADS;
+    if (split.rows_per_block > 1) {
+        local = v / split.vecs;
+        v -= local * split.vecs;
+    }
+    const long long t = (long long)blockIdx.x * split.rows_per_block + local;
+    if (local >= split.rows_per_block || v >= split.vecs || t >= tokens) return;
+    const long long D = (long long)split.vecs * N;
+    float acc[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    float rest = 1.f;
+    for (int s = 0; s < k; ++s) {
+        const long long slot = t * k + s;
+        const long long row = row_of ? row_of[slot] : slot;
+        if (row < 0 || row >= rows || (gate && (unsigned)gate[slot] >= gates)) continue;
+        const float w = weight[slot];
+        rest -= w;
+        float e[N];
+        load_elems<T, N>(y + row * D + (long long)v * N, e);
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = fmaf(w, e[i], acc[i]);
+    }
+    if (RESIDUAL) {
+        float e[N];
+        load_elems<T, N>(x + t * D + (long long)v * N, e);
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = fmaf(rest, e[i], acc[i]);
+    }
+    store_elems<T, N>(out + t * D + (long long)v * N, acc);
+}
+
+bool aligned(const void* p, size_t bytes) { return ((uintptr_t)p % bytes) == 0; }
+
+RowSplit row_split(long long vecs) {
+    return RowSplit{(int)vecs, vecs >= ROW_THREADS ? 1 : (int)(ROW_THREADS / vecs)};
+}
+dim3 row_split_grid(const RowSplit& s, long long rows) {
+    return dim3((unsigned)((rows + s.rows_per_block - 1) / s.rows_per_block),
+                s.rows_per_block > 1 ? 1u : (unsigned)((s.vecs + ROW_THREADS - 1) / ROW_THREADS));
+}
+
+template <typename Vec>
+int launch_scatter_topk_vec(long long rows, int k, long long row_bytes, const void* x, long long ldx_bytes, const int* pos,
+                            const int* valid_rows, void* routed, int* row_of, cudaStream_t stream) {
+    const RowSplit s = row_split(row_bytes / (long long)sizeof(Vec));
+    INFMOE_CUDA_TRY(launch_chained_2d(scatter_topk_kernel<Vec>, row_split_grid(s, rows), ROW_THREADS, stream, rows, k, s,
+                                      (const Vec*)x, ldx_bytes / (long long)sizeof(Vec), pos, valid_rows, (Vec*)routed, row_of));
+    note_launch();
+    INFMOE_CUDA_TRY(cudaGetLastError());
+    return INFMOE_OK;
+}
+
+template <typename T, int N>
+int launch_combine_topk_vec(long long tokens, int k, int D, const void* y, long long rows, const float* weight, const int* gate,
+                            unsigned gates, const int* row_of, const void* x, void* out, cudaStream_t stream) {
+    const RowSplit s = row_split(D / N);
+    const dim3 grid = row_split_grid(s, tokens);
+    if (x)
+        INFMOE_CUDA_TRY(launch_chained_2d(combine_topk_kernel<T, N, true>, grid, ROW_THREADS, stream, tokens, k, s, (const T*)y,
+                                          rows, weight, gate, gates, row_of, (const T*)x, (T*)out));
+    else
+        INFMOE_CUDA_TRY(launch_chained_2d(combine_topk_kernel<T, N, false>, grid, ROW_THREADS, stream, tokens, k, s,
+                                          (const T*)y, rows, weight, gate, gates, row_of, (const T*)x, (T*)out));
+    note_launch();
+    INFMOE_CUDA_TRY(cudaGetLastError());
+    return INFMOE_OK;
+}
+
+template <typename T>
+int launch_combine_topk_type(long long tokens, int k, int D, const void* y, long long rows, const float* weight,
+                             const int* gate, unsigned gates, const int* row_of, const void* x, void* out, cudaStream_t stream) {
+    constexpr int N = 16 / (int)sizeof(T);
+    if (D % N == 0 && aligned(y, 16) && aligned(out, 16) && (!x || aligned(x, 16)))
+        return launch_combine_topk_vec<T, N>(tokens, k, D, y, rows, weight, gate, gates, row_of, x, out, stream);
+    return launch_combine_topk_vec<T, 1>(tokens, k, D, y, rows, weight, gate, gates, row_of, x, out, stream);
+}
+
+}  // namespace
+
+int launch_scatter_topk(long long rows, int k, int D, int elem_bytes, const void* x, long long ldx, const int* pos,
+                        const int* valid_rows, void* routed, int* row_of, cudaStream_t stream) {
+    const long long row_bytes = (long long)D * elem_bytes, ldx_bytes = ldx * elem_bytes;
+    if (row_bytes % 16 == 0 && ldx_bytes % 16 == 0 && aligned(x, 16) && aligned(routed, 16))
+        return launch_scatter_topk_vec<uint4>(rows, k, row_bytes, x, ldx_bytes, pos, valid_rows, routed, row_of, stream);
+    if (elem_bytes == 4)
+        return launch_scatter_topk_vec<uint32_t>(rows, k, row_bytes, x, ldx_bytes, pos, valid_rows, routed, row_of, stream);
+    return launch_scatter_topk_vec<uint16_t>(rows, k, row_bytes, x, ldx_bytes, pos, valid_rows, routed, row_of, stream);
+}
+
+int launch_combine_topk(long long tokens, int k, int D, int dtype, const void* y, long long rows, const float* weight,
+                        const int* gate, unsigned gates, const int* row_of, const void* x, void* out, cudaStream_t stream) {
+    if (dtype == INFMOE_F32)
+        return launch_combine_topk_type<float>(tokens, k, D, y, rows, weight, gate, gates, row_of, x, out, stream);
+    if (dtype == INFMOE_F16)
+        return launch_combine_topk_type<__half>(tokens, k, D, y, rows, weight, gate, gates, row_of, x, out, stream);
+    return launch_combine_topk_type<__nv_bfloat16>(tokens, k, D, y, rows, weight, gate, gates, row_of, x, out, stream);
+}
+
+}  // namespace infmoe
+
+using namespace infmoe;
+
+extern "C" {
+
+int infmoe_expert_select_topk(const infmoe_topk_config* cfg, int64_t T, const void* d_logits, int32_t dtype, int64_t ld,
+                              const float* d_bias, int32_t* d_gate, float* d_weight, int32_t* d_status, void* stream) {
+    if (!cfg || T < 0 || T > 0x7fffffffLL || !known_dtype(dtype) || (T > 0 && (!d_logits || !d_gate || !d_weight))) {
+        set_error("expert_select_topk: bad argument (T=%lld dtype=%d)", (long long)T, dtype);
+        return INFMOE_ERR_INVALID_ARGUMENT;
+    }
+    const int E = cfg->expert_count, k = cfg->top_k, G = cfg->group_count;
+    if (E <= 0 || ld < E || G <= 0 || G > E || E % G != 0 || cfg->top_groups <= 0 || cfg->top_groups > G || k <= 0 ||
+        (int64_t)k > (int64_t)cfg->top_groups * (E / G) || (cfg->group_best != 1 && cfg->group_best != 2) ||
+        (cfg->score != INFMOE_SCORE_SOFTMAX && cfg->score != INFMOE_SCORE_SIGMOID)) {
+        set_error("expert_select_topk: bad configuration (experts %d, groups %d, top groups %d, top_k %d, best of a group %d, "
+                  "score %d, row stride %lld)", E, G, cfg->top_groups, k, cfg->group_best, cfg->score, (long long)ld);
+        return INFMOE_ERR_INVALID_ARGUMENT;
+    }
+    int padded = 1;
+    while (padded < G) padded *= 2;
+    const int size = E / G, lanes = padded <= 32 ? 32 / padded : 0;
+    if (k > 32 || lanes == 0 || (size + lanes - 1) / lanes > 32) {
+        set_error("expert_select_topk: at most 32 experts to a token, 32 groups and 32 experts to a lane (experts %d, groups %d, "
+                  "top_k %d)", E, G, k);
+        return INFMOE_ERR_UNSUPPORTED;
+    }
+    if (T == 0) return INFMOE_OK;
+    SelectArgs a{};
+    a.logits = d_logits;
+    a.T = T;
+    a.ld = ld;
+    a.E = E;
+    a.k = k;
+    a.groups = G;
+    a.top_groups = cfg->top_groups;
+    a.group_best = cfg->group_best;
+    a.group_size = size;
+    a.lanes = lanes;
+    a.sigmoid = cfg->score == INFMOE_SCORE_SIGMOID;
+    a.renormalise = cfg->renormalise != 0;
+    a.scale = cfg->scale;
+    a.bias = d_bias;
+    a.gate = d_gate;
+    a.weight = d_weight;
+    a.status = d_status;
+    const int per_lane = (size + lanes - 1) / lanes;
+    if (dtype == INFMOE_F32) return launch_select_type<float>(a, per_lane, (cudaStream_t)stream);
+    if (dtype == INFMOE_F16) return launch_select_type<__half>(a, per_lane, (cudaStream_t)stream);
+    return launch_select_type<__nv_bfloat16>(a, per_lane, (cudaStream_t)stream);
+}
+
+int infmoe_expert_scatter_topk(int64_t T, int32_t top_k, int32_t token_len, int32_t dtype, const void* d_input, int64_t ld,
+                               const int32_t* d_pos, const int32_t* d_valid_rows, void* d_routed, int32_t* d_row_of,
+                               void* stream) {
+    if (T < 0 || top_k <= 0 || token_len <= 0 || ld < token_len || !known_dtype(dtype) ||
+        (T > 0 && (!d_input || !d_pos || !d_valid_rows || !d_routed))) {
+        set_error("expert_scatter_topk: bad argument (T=%lld top_k=%d token_len=%d row stride %lld dtype=%d)", (long long)T, top_k,
+                  token_len, (long long)ld, dtype);
+        return INFMOE_ERR_INVALID_ARGUMENT;
+    }
+    if (T > 0x7fffffffLL / top_k) {
+        set_error("expert_scatter_topk: %lld tokens of %d slots are too many for 32-bit slot indices", (long long)T, top_k);
+        return INFMOE_ERR_UNSUPPORTED;
+    }
+    if (T == 0) return INFMOE_OK;
+    return launch_scatter_topk(T * top_k, top_k, token_len, dtype_bytes(dtype), d_input, ld, d_pos, d_valid_rows, d_routed,
+                               d_row_of, (cudaStream_t)stream);
+}
+
+int infmoe_expert_combine_topk(int64_t T, int32_t top_k, int32_t token_len, int32_t dtype, const void* d_rows, int64_t rows,
+                               const float* d_weight, const int32_t* d_gate, const int32_t* d_row_of, const void* d_residual,
+                               void* d_output, void* stream) {
+    if (T < 0 || rows < 0 || top_k <= 0 || token_len <= 0 || !known_dtype(dtype) ||
+        (T > 0 && ((rows > 0 && !d_rows) || !d_weight || !d_output)) || (T > 0 && d_rows == d_output)) {
+        set_error("expert_combine_topk: bad argument (T=%lld rows=%lld top_k=%d token_len=%d dtype=%d)", (long long)T,
+                  (long long)rows, top_k, token_len, dtype);
+        return INFMOE_ERR_INVALID_ARGUMENT;
+    }
+    if (T > 0x7fffffffLL / top_k) {
+        set_error("expert_combine_topk: %lld tokens of %d slots are too many for 32-bit slot indices", (long long)T, top_k);
+        return INFMOE_ERR_UNSUPPORTED;
+    }
+    if (T == 0) return INFMOE_OK;
+    return launch_combine_topk(T, top_k, token_len, dtype, d_rows, rows, d_weight, d_gate, 0x80000000u, d_row_of, d_residual,
+                               d_output, (cudaStream_t)stream);
+}
+
+}  // extern "C"

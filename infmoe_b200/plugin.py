@@ -296,14 +296,18 @@ class MoELayer:
         return int(capi.lib().infmoe_layer_kernel_launches(self._h))
 
     # -- conveniences ---------------------------------------------------------------------------
-    def forward(self, x, out=None, stream: Optional[int] = None):
-        """x: CUDA float32 torch tensor [..., D]; returns a tensor of the same shape (stream ordered)."""
+    def forward(self, x, out=None, stream: Optional[int] = None, adapters=None, plan=None):
+        """x: CUDA float32 torch tensor [..., D]; returns a tensor of the same shape (stream ordered).
+
+        adapters, plan: low-rank adapters of the tokens' requests (Adapters, AdapterPlan), added to the layer's output."""
         # A small layer's pass is no longer than the calls that issue it, so this one asks for little: of 20 us for 32 tokens, 4
         # experts, 64 x 256, reading embedding_size through the C ABI and making a torch.cuda.Stream object took about 4.
         import torch
 
         if not (x.is_cuda and x.dtype == torch.float32 and x.is_contiguous()):
             raise ValueError("x must be a contiguous float32 CUDA tensor")
+        if (adapters is None) != (plan is None):
+            raise ValueError("adapters need the plan of the batch, and a plan its adapters")
         T = x.numel() // self.embedding_size
         if out is None:
             out = torch.empty_like(x)
@@ -312,6 +316,41 @@ class MoELayer:
             self._ws = torch.empty(need, dtype=torch.uint8, device=x.device)
         s = _current_stream(torch, x.get_device()) if stream is None else stream
         self.enqueue(x.data_ptr(), out.data_ptr(), self._ws.data_ptr(), self._ws.numel(), T, s)
+        if adapters is not None:
+            if stream is not None:
+                with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=x.device)):
+                    return adapters.apply(x, out, plan, out=out)
+            adapters.apply(x, out, plan, out=out)
+        return out
+
+    def forward_topk(self, x, gate, weight, out=None):
+        """x: CUDA float32 tensor [..., D], each of whose tokens goes to the experts gate [..., k] (int32; an index outside
+        [0, expert_count): none) with the weights weight [..., k] (float32): x + sum_s weight_s (E_s(x) - x).
+
+        gate and weight are what TopKRouter.select returns.  On torch's current stream; the workspace comes from torch's
+        allocator and goes back to it."""
+        import torch
+
+        from .topk import check_array, launch
+
+        if not (x.is_cuda and x.dtype == torch.float32 and x.is_contiguous() and x.dim() >= 1 and
+                x.shape[-1] == self.embedding_size):
+            raise ValueError(f"x must be a contiguous float32 CUDA tensor [..., {self.embedding_size}]")
+        if gate.dim() < 1 or gate.shape[-1] < 1:
+            raise ValueError("gate must be [..., k]")
+        k = gate.shape[-1]
+        check_array(gate, (*x.shape[:-1], k), torch.int32, x.device, "gate")
+        check_array(weight, (*x.shape[:-1], k), torch.float32, x.device, "weight")
+        if out is None:
+            out = torch.empty_like(x)
+        else:
+            check_array(out, x.shape, torch.float32, x.device, "out")
+        T = x.numel() // self.embedding_size
+        need = ctypes.c_size_t()
+        capi.check(capi.lib().infmoe_layer_topk_workspace_bytes(self._h, T, k, ctypes.byref(need)))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=x.device)
+        launch(x.get_device(), "infmoe_layer_forward_topk", self._h, x.data_ptr(), gate.data_ptr(), weight.data_ptr(), T, k,
+               out.data_ptr(), ws.data_ptr(), need.value)
         return out
 
     def forward_host(self, x: np.ndarray, out: Optional[np.ndarray] = None) -> np.ndarray:

@@ -1,0 +1,204 @@
+"""Several experts per token: routing to the k best, rows to their experts and back (torch tensors over the C ABI).
+
+    router = TopKRouter(expert_count, top_k, score="sigmoid", bias=bias, groups=8, top_groups=4)
+    gate, weight = router.select(logits)                              # the gate's projection of the tokens, [T, E]
+    pos, count, offset = count_experts(gate, expert_count)
+    routed, row_of = scatter_topk(x, pos, offset, top_k)              # rows in expert order, for experts of your own
+    out = combine_topk(results, weight, row_of=row_of)
+
+`MoELayer.forward_topk(x, gate, weight)` runs a layer's own experts in the place of the last three lines.  The reference routes
+every token to one expert (top-k is a TODO there).
+
+All functions work on torch's current stream of the tensors' device, and allocate what they return unless they are given it.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+from . import capi
+
+__all__ = ["TopKRouter", "count_experts", "scatter_topk", "combine_topk"]
+
+_DTYPES = {}
+
+
+def dtype_code(t) -> int:
+    """infmoe_dtype of a tensor; ValueError for types the library does not take."""
+    if not _DTYPES:
+        import torch
+
+        _DTYPES.update({torch.float32: capi.DTYPE_F32, torch.float16: capi.DTYPE_F16, torch.bfloat16: capi.DTYPE_BF16})
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"tensors of {t.dtype} are not supported: use float32, float16 or bfloat16")
+    return code
+
+
+def launch(device: int, name: str, *args) -> None:
+    """Calls a C entry point whose last argument is the stream, on `device` and torch's current stream there."""
+    import torch
+
+    from .plugin import _current_stream
+
+    fn = getattr(capi.lib(), name)
+    if torch.cuda.current_device() == device:
+        capi.check(fn(*args, _current_stream(torch, device)))
+    else:
+        with torch.cuda.device(device):
+            capi.check(fn(*args, _current_stream(torch, device)))
+
+
+def rows_of(t, width: int, what: str) -> Tuple[int, int]:
+    """(rows, row stride) of a CUDA tensor [..., width]: rows apart by any stride for [T, width], contiguous otherwise."""
+    if not t.is_cuda or t.dim() < 1 or t.shape[-1] != width or (width > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{what} must be a CUDA tensor [..., {width}] with consecutive elements in a row")
+    rows = t.numel() // width
+    if t.dim() == 2 and rows > 1:
+        ld = t.stride(0)
+        if ld < width:
+            raise ValueError(f"the rows of {what} overlap (stride {ld})")
+        return rows, ld
+    if t.dim() > 2 and not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous (or two-dimensional)")
+    return rows, width
+
+
+def check_array(t, shape, dtype, device, what: str) -> None:
+    """A contiguous tensor of this shape and type on this device."""
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous {str(dtype)[6:]} tensor of shape {list(shape)} on {device}")
+
+
+class TopKRouter:
+    """The choice of a token's k experts from its gating logits (infmoe_expert_select_topk).
+
+    score        "softmax" or "sigmoid" of the logits
+    bias         float32 CUDA tensor [expert_count] added to the scores for the choice alone (load balance), or None;
+                 read at every call, so it may be updated in place
+    groups, top_groups, group_best
+                 with groups > 1, only the experts of the top_groups best groups are chosen from; a group counts with the sum
+                 of its two best experts (group_best=2) or with its best one (1)
+    renormalise  the weights of a token's experts sum to `scale`
+    """
+
+    def __init__(self, expert_count: int, top_k: int, score: str = "softmax", bias=None, groups: int = 1, top_groups: int = 1,
+                 group_best: int = 1, renormalise: bool = True, scale: float = 1.0) -> None:
+        import torch
+
+        if score not in capi.SCORES:
+            raise ValueError(f"score must be one of {sorted(capi.SCORES)}")
+        if bias is not None and not (bias.is_cuda and bias.dtype == torch.float32 and tuple(bias.shape) == (expert_count,) and
+                                     bias.is_contiguous()):
+            raise ValueError(f"bias must be a contiguous float32 CUDA tensor of shape [{expert_count}]")
+        self.expert_count, self.top_k, self.bias = int(expert_count), int(top_k), bias
+        self._cfg = capi.TopKConfig(expert_count, top_k, capi.SCORES[score], groups, top_groups, group_best, int(renormalise),
+                                    scale)
+        self._cfg_ref = ctypes.byref(self._cfg)
+        # what a configuration can be refused for, now and not at the first call: no tokens, no device work
+        capi.check(capi.lib().infmoe_expert_select_topk(self._cfg_ref, 0, None, capi.DTYPE_F32, expert_count, None, None, None,
+                                                        None, None))
+
+    def select(self, logits, gate=None, weight=None, status=None):
+        """logits: float32, float16 or bfloat16 CUDA tensor [..., expert_count] -> (gate int32, weight float32), [..., top_k].
+
+        Experts with a logit of NaN or of the type's lowest value or less (-inf) are not chosen; places that stay empty hold
+        gate -1 and weight 0.  status (int32 [1], may be None): bit 0 is set when a token has no expert at all."""
+        import torch
+
+        T, ld = rows_of(logits, self.expert_count, "logits")
+        code, device, k = dtype_code(logits), logits.device, self.top_k
+        if self.bias is not None and self.bias.device != device:
+            raise ValueError(f"logits are on {device}, the router's bias on {self.bias.device}")
+        shape = (*logits.shape[:-1], k)
+        if gate is None:
+            gate = torch.empty(shape, dtype=torch.int32, device=device)
+        else:
+            check_array(gate, shape, torch.int32, device, "gate")
+        if weight is None:
+            weight = torch.empty(shape, dtype=torch.float32, device=device)
+        else:
+            check_array(weight, shape, torch.float32, device, "weight")
+        if status is not None:
+            check_array(status, (1,), torch.int32, device, "status")
+        launch(logits.get_device(), "infmoe_expert_select_topk", self._cfg_ref, T, logits.data_ptr(), code, ld,
+               self.bias.data_ptr() if self.bias is not None else None, gate.data_ptr(), weight.data_ptr(),
+               status.data_ptr() if status is not None else None)
+        return gate, weight
+
+
+def count_experts(gate, expert_count: int, status=None):
+    """gate: int32 CUDA tensor of expert indices, one per slot -> (pos, count, offset) of the slots in expert order
+    (infmoe_expert_count).  Slots with an index outside [0, expert_count) come last, offset[expert_count] is where they begin;
+    status (int32 [1], may be None): bit 1 is set when there are any."""
+    import torch
+
+    if not gate.is_cuda or gate.dtype != torch.int32 or not gate.is_contiguous():
+        raise ValueError("gate must be a contiguous int32 CUDA tensor")
+    pos = torch.empty(gate.numel(), dtype=torch.int32, device=gate.device)
+    count = torch.empty(expert_count, dtype=torch.int32, device=gate.device)
+    offset = torch.empty(expert_count + 1, dtype=torch.int32, device=gate.device)
+    if status is not None:
+        check_array(status, (1,), torch.int32, gate.device, "status")
+    launch(gate.get_device(), "infmoe_expert_count", gate.numel(), expert_count, gate.data_ptr(), pos.data_ptr(),
+           count.data_ptr(), offset.data_ptr(), status.data_ptr() if status is not None else None)
+    return pos, count, offset
+
+
+def scatter_topk(x, pos, offset, top_k: int, out=None, row_of=None):
+    """x [..., D] -> (rows in expert order [T * top_k, D], row of every slot [T, top_k], -1 for slots without an expert).
+
+    pos and offset are count_experts' of the slots; rows behind the last expert's are left as they are in `out`."""
+    import torch
+
+    D = x.shape[-1]
+    T, ld = rows_of(x, D, "x")
+    slots, device = T * top_k, x.device
+    check_array(pos, (slots,), torch.int32, device, "pos")
+    if offset.dim() != 1 or offset.numel() < 1:
+        raise ValueError("offset must hold expert_count + 1 row numbers")
+    check_array(offset, offset.shape, torch.int32, device, "offset")
+    if out is None:
+        out = torch.empty((slots, D), dtype=x.dtype, device=device)
+    else:
+        check_array(out, (slots, D), x.dtype, device, "out")
+    if row_of is None:
+        row_of = torch.empty((T, top_k), dtype=torch.int32, device=device)
+    else:
+        check_array(row_of, (T, top_k), torch.int32, device, "row_of")
+    launch(x.get_device(), "infmoe_expert_scatter_topk", T, top_k, D, dtype_code(x), x.data_ptr(), ld, pos.data_ptr(),
+           offset.data_ptr() + 4 * (offset.numel() - 1), out.data_ptr(), row_of.data_ptr())
+    return out, row_of
+
+
+def combine_topk(rows, weight, row_of=None, gate=None, residual=None, out=None):
+    """out[t] = sum_s weight[t, s] * rows[row_of[t, s]] (+ (1 - sum_s weight[t, s]) * residual[t]).
+
+    rows [n, D]; weight float32 [..., top_k]; row_of int32 like weight (None: slot (t, s) is row t * top_k + s); gate int32
+    like weight or None: slots with a negative gate are left out, like slots whose row lies outside [0, n).  residual, out:
+    [..., D] like weight's leading dimensions; out may be residual."""
+    import torch
+
+    device = rows.device
+    if rows.dim() != 2 or not rows.is_cuda or not rows.is_contiguous():
+        raise ValueError("rows must be a contiguous CUDA tensor [n, D]")
+    n, D = rows.shape
+    if weight.dim() < 1:
+        raise ValueError("weight must be [..., top_k]")
+    k = weight.shape[-1]
+    check_array(weight, weight.shape, torch.float32, device, "weight")
+    T = weight.numel() // k if k else 0
+    shape = (*weight.shape[:-1], D)
+    for t, what in ((row_of, "row_of"), (gate, "gate")):
+        if t is not None:
+            check_array(t, weight.shape, torch.int32, device, what)
+    if residual is not None:
+        check_array(residual, shape, rows.dtype, device, "residual")
+    if out is None:
+        out = torch.empty(shape, dtype=rows.dtype, device=device)
+    else:
+        check_array(out, shape, rows.dtype, device, "out")
+    launch(rows.get_device(), "infmoe_expert_combine_topk", T, k, D, dtype_code(rows), rows.data_ptr(), n, weight.data_ptr(),
+           gate.data_ptr() if gate is not None else None, row_of.data_ptr() if row_of is not None else None,
+           residual.data_ptr() if residual is not None else None, out.data_ptr())
+    return out

@@ -1,0 +1,237 @@
+"""Low-rank adapters of many requests beside a shared projection, against a 64-bit reference (tests/topk_ref.py)."""
+import numpy as np
+import pytest
+import torch
+
+from infmoe_b200 import AdapterPlan, Adapters, synth
+from tests import topk_ref
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def whole(rng, shape, most, dtype):
+    return torch.from_numpy(rng.integers(-most, most + 1, size=shape).astype(np.float32)).cuda().to(dtype)
+
+
+def owners(rng, T, n, requests, none=0.15):
+    """Requests one behind the other, some of them with an index that means no adapter."""
+    ends = np.sort(rng.integers(0, T + 1, size=requests - 1)) if requests < T else np.arange(1, T)
+    which = rng.integers(0, n, size=requests).astype(np.int32)
+    which[rng.random(requests) < none] = rng.choice([-1, n, n + 5, -9])
+    return which[np.searchsorted(ends, np.arange(T), side="right")]
+
+
+def reference(x, y, a, b, scale, rank, at):
+    d = lambda v: None if v is None else v.double().cpu().numpy()  # noqa: E731
+    n = a.shape[0]
+    s = np.full(n, float(scale)) if isinstance(scale, (int, float)) else d(scale)
+    return topk_ref.adapters(d(x), d(y), d(a), d(b), s, None if rank is None else rank.cpu().numpy(), at)
+
+
+def check_exact(got, want, dtype):
+    """Sums of whole numbers, exact in 32 bits whatever their order: only the last rounding is left."""
+    assert torch.equal(got.cpu(), torch.from_numpy(want).to(dtype)), \
+        np.abs(got.double().cpu().numpy() - torch.from_numpy(want).to(dtype).double().numpy()).max()
+
+
+# Whole numbers: |A x| <= 4 d_in in whole numbers, |B v| below 2^24; rounding to the type is the last step alone.
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,n,r,d_in,d_out,requests", [
+    (1, 1, 1, 1, 1, 1), (1, 1, 16, 64, 64, 1), (1, 3, 8, 4096, 4096, 1), (2, 2, 3, 7, 5, 2), (16, 4, 16, 256, 512, 16),
+    (17, 2, 8, 100, 36, 3), (63, 5, 24, 510, 130, 7), (64, 1, 64, 1024, 256, 1), (65, 1, 33, 128, 1000, 1),
+    (130, 3, 128, 520, 264, 3), (200, 9, 4, 1000, 2724, 31), (300, 40, 17, 72, 80, 100), (64, 64, 16, 2048, 2048, 64),
+    (700, 2, 48, 1028, 516, 4), (37, 1000, 8, 64, 64, 37), (513, 6, 10, 96, 4100, 9), (5, 2, 127, 33, 2050, 2),
+    (256, 2, 65, 192, 130, 2), (20, 3, 16, 10240, 64, 5)])
+def test_whole_numbers(T, n, r, d_in, d_out, requests, dtype):
+    rng = np.random.default_rng(T * 7 + r)
+    t = TYPES[dtype]
+    x, a = whole(rng, (T, d_in), 2, t), whole(rng, (n, r, d_in), 2, t)
+    b, y = whole(rng, (n, d_out, r), 1, t), whole(rng, (T, d_out), 50, t)
+    at = owners(rng, T, n, requests)
+    scale = torch.from_numpy(2.0 ** rng.integers(-3, 1, size=n).astype(np.float32)).cuda()
+    adapters = Adapters(a, b, scale=scale)
+    plan = adapters.plan(torch.from_numpy(at).cuda())
+    want = reference(x, y, a, b, scale, None, at)
+    check_exact(adapters.apply(x, y, plan), want, t)
+    inplace = y.clone()
+    assert adapters.apply(x, inplace, plan, out=inplace) is inplace
+    check_exact(inplace, want, t)
+    rank = torch.from_numpy(rng.integers(-1, r + 3, size=n).astype(np.int32)).cuda()
+    check_exact(Adapters(a, b, scale, rank).apply(x, y, plan), reference(x, y, a, b, scale, rank, at), t)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,n,r,d_in,d_out", [(50, 3, 16, 4096, 1024), (300, 7, 64, 1000, 700), (9, 9, 8, 512, 10240),
+                                              (1, 1, 128, 2050, 2050)])
+def test_against_64_bits(T, n, r, d_in, d_out, dtype):
+    """The products in at least 32 bits.  The error of a sum of d_in rounded products, taken as a random walk of half units, is
+    sqrt(d_in) 2^-24 of its terms' 2-norm, which for terms of one size is that of the sum times 2^-24 sqrt(d_in); eight times
+    that (a chain of adds that truncates is twice as bad, and so is a walk at four sigma) covers A x, and B v with r for d_in.
+    With v kept in two parts of 8 bits each its own rounding is 2^-17, so 16-bit types get that too, and the stored half unit."""
+    rng = np.random.default_rng(r)
+    t = TYPES[dtype]
+    f = lambda *s: torch.from_numpy(rng.standard_normal(s)).cuda()  # noqa: E731
+    x, y = f(T, d_in).to(t), torch.zeros(T, d_out, device="cuda", dtype=t)
+    a, b = (f(n, r, d_in) / d_in ** 0.5).to(t), (f(n, d_out, r) / r ** 0.5).to(t)
+    at = rng.integers(0, n, size=T).astype(np.int32)
+    adapters = Adapters(a, b, scale=0.75)
+    got = adapters.apply(x, y, adapters.plan(torch.from_numpy(at).cuda())).double().cpu().numpy()
+    want = reference(x, y, a, b, 0.75, None, at)
+    eps = {"f32": 2.0 ** -24, "f16": 2.0 ** -11 + 2.0 ** -17, "bf16": 2.0 ** -8 + 2.0 ** -17}[dtype]
+    tol = 8 * 2.0 ** -24 * (d_in ** 0.5 + r ** 0.5) + eps
+    assert np.linalg.norm(got - want) <= tol * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_apart_and_unaligned(dtype):
+    rng = np.random.default_rng(4)
+    t = TYPES[dtype]
+    T, n, r, d_in, d_out = 90, 3, 16, 128, 256
+    xs, ys = whole(rng, (T, d_in + 9), 2, t), whole(rng, (T, d_out + 9), 50, t)
+    a, b = whole(rng, (n, r, d_in), 2, t), whole(rng, (n, d_out, r), 1, t)
+    at = owners(rng, T, n, 5)
+    adapters = Adapters(a, b)
+    plan = adapters.plan(torch.from_numpy(at).cuda())
+    for i, j in ((0, 0), (1, 0), (0, 3), (8, 8)):
+        x, y = xs[:, i:i + d_in], ys[:, j:j + d_out]
+        want = reference(x, y, a, b, 1, None, at)
+        check_exact(adapters.apply(x, y, plan), want, t)
+        outs = torch.full((T + 2, d_out + 5), 9.0, device="cuda", dtype=t)
+        adapters.apply(x, y, plan, out=outs[:T, 2:2 + d_out])
+        check_exact(outs[:T, 2:2 + d_out], want, t)
+        assert (outs[T:] == 9).all() and (outs[:, :2] == 9).all() and (outs[:, 2 + d_out:] == 9).all()
+        keep = ys.clone()
+        adapters.apply(x, keep[:, j:j + d_out], plan, out=keep[:, j:j + d_out])
+        check_exact(keep[:, j:j + d_out], want, t)
+        assert torch.equal(keep[:, :j], ys[:, :j]) and torch.equal(keep[:, j + d_out:], ys[:, j + d_out:])
+
+
+def test_weights_that_start_between_boundaries():
+    rng = np.random.default_rng(6)
+    n, r, d_in, d_out, T = 2, 8, 64, 72, 40
+    fa, fb = whole(rng, (n * r * d_in + 1,), 2, torch.bfloat16), whole(rng, (n * r * d_out + 1,), 1, torch.bfloat16)
+    a, b = fa[1:].view(n, r, d_in), fb[1:].view(n, d_out, r)
+    x, y = whole(rng, (T, d_in), 2, torch.bfloat16), whole(rng, (T, d_out), 9, torch.bfloat16)
+    at = owners(rng, T, n, 4)
+    adapters = Adapters(a, b)
+    check_exact(adapters.apply(x, y, adapters.plan(torch.from_numpy(at).cuda())), reference(x, y, a, b, 1, None, at),
+                torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_nobody_elses_numbers(dtype):
+    """Rows of tokens without an adapter pass as they are, with what they hold; infinities and NaN stay in their own rows and in
+    the adapters that nobody uses, and so does what lies past an adapter's rank."""
+    rng = np.random.default_rng(9)
+    t = TYPES[dtype]
+    T, n, r, d_in, d_out = 80, 4, 16, 200, 136
+    x, y = whole(rng, (T, d_in), 2, t), whole(rng, (T, d_out), 50, t)
+    a, b = whole(rng, (n, r, d_in), 2, t), whole(rng, (n, d_out, r), 1, t)
+    at = np.array([0, 1, -1, 3] * 20, np.int32)
+    at[5] = -1
+    rank = torch.tensor([16, 5, 16, 16], dtype=torch.int32, device="cuda")
+    want = reference(x, y, a, b, 1, rank, at)
+    a[2], b[2] = np.nan, np.inf                                     # nobody's adapter
+    a[1, 5:], b[1, :, 5:] = np.nan, np.nan                          # past its rank
+    x[2], x[6], x[10] = np.nan, np.inf, torch.finfo(t).max          # of tokens without an adapter
+    y[2], y[6] = np.nan, -np.inf
+    x[4, 3] = np.nan                                                # a token of adapter 0
+    adapters = Adapters(a, b, rank=rank)
+    got = adapters.apply(x, y, adapters.plan(torch.from_numpy(at).cuda()))
+    rest = np.setdiff1d(np.arange(T), [2, 4, 6])
+    check_exact(got[rest], want[rest], t)
+    assert torch.isnan(got[2]).all() and (got[6] == -np.inf).all() and torch.isnan(got[4]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_large_and_small_inner_values(dtype):
+    """A x far above and below what 16 bits hold, brought back by B and the scale."""
+    rng = np.random.default_rng(12)
+    t = TYPES[dtype]
+    T, r, d_in, d_out = 33, 16, 512, 64
+    for up, down in ((2.0 ** 7, 2.0 ** -12), (2.0 ** -10, 2.0 ** 8)):
+        x, a = whole(rng, (T, d_in), 2, t) * up, whole(rng, (1, r, d_in), 2, t) * up
+        b, y = whole(rng, (1, d_out, r), 1, t) * down, torch.zeros(T, d_out, device="cuda", dtype=t)
+        at = np.zeros(T, np.int32)
+        scale = torch.full((1,), up ** -2, device="cuda")
+        adapters = Adapters(a, b, scale=scale)
+        check_exact(adapters.apply(x, y, adapters.plan(torch.from_numpy(at).cuda())),
+                    reference(x, y, a, b, scale, None, at), t)
+
+
+def test_plans():
+    rng = np.random.default_rng(2)
+    x, y = whole(rng, (200, 64), 2, torch.float32), whole(rng, (200, 64), 9, torch.float32)
+    a, b = whole(rng, (5, 8, 64), 2, torch.float32), whole(rng, (5, 64, 8), 1, torch.float32)
+    adapters = Adapters(a, b)
+    for at in (np.full(200, -1), np.full(200, 4), np.arange(200) % 5, np.arange(200) % 6 - 1):
+        at = at.astype(np.int32)
+        plan = AdapterPlan(torch.from_numpy(at).cuda(), 5)
+        check_exact(adapters.apply(x, y, plan), reference(x, y, a, b, 1, None, at), torch.float32)
+    empty = adapters.plan(torch.empty(0, dtype=torch.int32, device="cuda"))
+    assert adapters.apply(x[:0], y[:0], empty).shape == (0, 64)
+    with pytest.raises(ValueError):
+        adapters.apply(x[:199], y[:199], plan)                      # another batch's plan
+    with pytest.raises(ValueError):
+        Adapters(a[:4].contiguous(), b[:4].contiguous()).apply(x, y, plan)
+    with pytest.raises(ValueError):
+        adapters.apply(x.double(), y, plan)
+    with pytest.raises(ValueError):
+        adapters.apply(x, y, plan, out=y[:199])
+    with pytest.raises(ValueError):
+        adapters.plan(torch.zeros(5, dtype=torch.int64, device="cuda"))
+    with pytest.raises(ValueError):
+        Adapters(a, b.half())
+    with pytest.raises(ValueError):
+        Adapters(a, b, scale=torch.ones(4, device="cuda"))
+
+
+def test_same_bits_every_time():
+    """No order that a run leaves open."""
+    rng = np.random.default_rng(3)
+    f = lambda *s: torch.from_numpy(rng.standard_normal(s)).cuda().to(torch.bfloat16)  # noqa: E731
+    n, r, d_in, d_out, T = 4, 16, 1024, 1024, 300
+    x, y, a, b = f(T, d_in), f(T, d_out), f(n, r, d_in), f(n, d_out, r)
+    at = torch.from_numpy(owners(rng, T, n, 12)).cuda()
+    adapters = Adapters(a, b)
+    first = adapters.apply(x, y, adapters.plan(at))
+    for _ in range(3):
+        assert torch.equal(adapters.apply(x, y, adapters.plan(at)), first)
+
+
+def test_layer_with_adapters_and_captured():
+    from tests.test_gpu_topk import small_layer
+
+    layer, _, xs = small_layer(4, 64, 128, variant="cpm_2", on_device=True)
+    rng = np.random.default_rng(1)
+    x = torch.from_numpy(xs).cuda()
+    f = lambda *s: torch.from_numpy(rng.standard_normal(s).astype(np.float32) * 0.1).cuda()  # noqa: E731
+    adapters = Adapters(f(3, 8, 64), f(3, 64, 8), scale=2.0)
+    at = torch.from_numpy(owners(rng, 70, 3, 6)).cuda()
+    plan = adapters.plan(at)
+    plain = layer.forward(x)
+    want = adapters.apply(x, plain, plan)
+    got = layer.forward(x, adapters=adapters, plan=plan)
+    assert torch.equal(got, want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    other = torch.empty_like(x)
+    side.wait_stream(torch.cuda.current_stream())
+    layer.forward(x, stream=side.cuda_stream, out=other, adapters=adapters, plan=plan)
+    torch.cuda.synchronize()
+    assert torch.equal(other, want)
+    with pytest.raises(ValueError):
+        layer.forward(x, adapters=adapters)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        p = adapters.plan(at)
+        out = layer.forward(x, adapters=adapters, plan=p)
+    x.mul_(0.5)
+    at.copy_(torch.from_numpy(owners(np.random.default_rng(5), 70, 3, 9)).cuda())
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, layer.forward(x, adapters=adapters, plan=adapters.plan(at)))
+    del g
+    layer.terminate()

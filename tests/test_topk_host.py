@@ -1,0 +1,145 @@
+"""What the operators for several experts per token and for adapters refuse, before any device work."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from infmoe_b200 import Adapters, TopKRouter, capi, combine_topk, count_experts, scatter_topk
+from tests import topk_ref
+
+GOOD = dict(expert_count=16, top_k=4, score=1, group_count=4, top_groups=2, group_best=2, renormalise=1, scale=1.0)
+SOME = 1 << 20      # an address that no refused call looks at
+
+
+def _select(T=3, logits=SOME, dtype=0, ld=16, gate=SOME, weight=SOME, cfg=None, **kw):
+    c = capi.TopKConfig(**{**GOOD, **kw})
+    ref = ctypes.byref(c) if cfg is None else cfg
+    return capi.lib().infmoe_expert_select_topk(ref, T, logits, dtype, ld, None, gate, weight, None, None)
+
+
+@pytest.mark.parametrize("bad", [dict(T=-1), dict(T=1 << 31), dict(logits=None), dict(gate=None), dict(weight=None),
+                                 dict(dtype=3), dict(dtype=-1), dict(ld=15), dict(expert_count=0), dict(expert_count=18, ld=18),
+                                 dict(top_k=0), dict(top_k=9), dict(group_count=0), dict(group_count=32, ld=32),
+                                 dict(top_groups=0), dict(top_groups=5), dict(group_best=0), dict(group_best=3), dict(score=2)],
+                         ids=str)
+def test_select_refuses_bad_arguments(bad):
+    assert _select(**bad) == 1 and "expert_select_topk" in capi.last_error()
+
+
+def test_select_refuses_what_no_kernel_has_lanes_for():
+    big = dict(group_count=1, top_groups=1, top_k=1)
+    assert _select(T=0, expert_count=1024, ld=1024, **big) == 0
+    assert _select(T=0, expert_count=1025, ld=1025, **big) == 6
+    assert _select(T=0, expert_count=64, ld=64, group_count=1, top_groups=1, top_k=33) == 6
+    assert _select(T=0, expert_count=66, ld=66, group_count=33, top_groups=1, top_k=1) == 6
+    assert _select(T=0, expert_count=17 * 33, ld=17 * 33, group_count=17, top_groups=1, top_k=1) == 6
+    assert _select(T=0) == 0
+    assert capi.lib().infmoe_expert_select_topk(None, 0, None, 0, 1, None, None, None, None, None) == 1
+
+
+@pytest.mark.parametrize("at,value,status", [(0, -1, 1), (1, 0, 1), (2, 0, 1), (3, 7, 1), (4, None, 1), (5, 7, 1), (6, None, 1),
+                                             (7, None, 1), (8, None, 1), (0, 1 << 30, 6)])
+def test_scatter_refuses_bad_arguments(at, value, status):
+    args = [3, 2, 8, 0, SOME, 8, SOME, SOME, SOME, SOME, None]
+    args[at] = value
+    assert capi.lib().infmoe_expert_scatter_topk(*args) == status
+
+
+@pytest.mark.parametrize("at,value,status", [(0, -1, 1), (1, 0, 1), (2, -8, 1), (3, 9, 1), (4, None, 1), (5, -1, 1), (6, None, 1),
+                                             (10, None, 1), (10, SOME, 1), (0, 1 << 30, 6)])
+def test_combine_refuses_bad_arguments(at, value, status):
+    args = [3, 2, 8, 0, SOME, 6, SOME, None, None, None, 2 * SOME, None]
+    args[at] = value
+    assert capi.lib().infmoe_expert_combine_topk(*args) == status
+
+
+def _apply(T=4, x=SOME, ldx=32, y=2 * SOME, ldy=48, out=3 * SOME, ldo=48, plan=4 * SOME, **kw):
+    s = capi.AdapterSet(**{**dict(adapter_count=3, rank=8, d_in=32, d_out=48, dtype=2, d_a=SOME, d_b=SOME), **kw})
+    return capi.lib().infmoe_adapter_apply(ctypes.byref(s), T, x, ldx, y, ldy, out, ldo, plan, None)
+
+
+@pytest.mark.parametrize("bad", [dict(T=-1), dict(x=None), dict(y=None), dict(out=None), dict(plan=None), dict(plan=8),
+                                 dict(ldx=31), dict(ldy=47), dict(ldo=47), dict(out=SOME), dict(out=2 * SOME, ldo=64),
+                                 dict(adapter_count=0), dict(rank=0), dict(d_in=0), dict(d_out=-1), dict(dtype=5),
+                                 dict(d_a=None), dict(d_b=None)], ids=str)
+def test_apply_refuses_bad_arguments(bad):
+    assert _apply(**bad) == 1 and "adapter_apply" in capi.last_error()
+
+
+def test_apply_refuses_what_is_too_large():
+    assert _apply(rank=capi.ADAPTER_MAX_RANK + 1) == 6
+    assert _apply(adapter_count=100000) == 6
+    assert _apply(T=1 << 31) == 6
+    assert _apply(T=0, rank=capi.ADAPTER_MAX_RANK) == 0
+
+
+def test_plan_refuses_bad_arguments():
+    lib, n = capi.lib(), ctypes.c_size_t()
+    assert lib.infmoe_adapter_plan_bytes(100, 7, ctypes.byref(n)) == 0
+    need = n.value
+    assert need >= 4 * 100 + 4 * 8 + 16 * 8
+    assert lib.infmoe_adapter_plan_bytes(100, 7, None) == 1
+    assert lib.infmoe_adapter_plan_bytes(-1, 7, ctypes.byref(n)) == 1
+    assert lib.infmoe_adapter_plan_bytes(100, 0, ctypes.byref(n)) == 1
+    assert lib.infmoe_adapter_plan_bytes(100, 100000, ctypes.byref(n)) == 6
+    assert lib.infmoe_adapter_plan(100, 7, SOME, SOME, need - 1, None) == 1 and str(need) in capi.last_error()
+    assert lib.infmoe_adapter_plan(100, 7, SOME, SOME + 4, need, None) == 1
+    assert lib.infmoe_adapter_plan(100, 7, None, SOME, need, None) == 1
+    assert lib.infmoe_adapter_plan(100, 7, SOME, None, need, None) == 1
+    assert lib.infmoe_adapter_plan(0, 7, None, None, 0, None) == 0
+
+
+def test_forward_topk_refuses_bad_arguments():
+    from tests.test_capi_host import _layer
+
+    layer, lib, n = _layer(), capi.lib(), ctypes.c_size_t()
+    assert lib.infmoe_layer_topk_workspace_bytes(layer._h, 10, 2, ctypes.byref(n)) == 0
+    need = n.value
+    assert need > layer.get_workspace_size(20) + 2 * 20 * 8 * 4
+    assert lib.infmoe_layer_topk_workspace_bytes(layer._h, 10, 0, ctypes.byref(n)) == 1
+    assert lib.infmoe_layer_topk_workspace_bytes(layer._h, -1, 2, ctypes.byref(n)) == 1
+    assert lib.infmoe_layer_topk_workspace_bytes(layer._h, 1 << 30, 2, ctypes.byref(n)) == 6
+    assert lib.infmoe_layer_topk_workspace_bytes(layer._h, 10, 2, None) == 1
+    good = [layer._h, SOME, SOME, SOME, 10, 2, 2 * SOME, 3 * SOME, need, None]
+    for at, value, status in [(0, None, 1), (1, None, 1), (2, None, 1), (3, None, 1), (4, -1, 1), (5, 0, 1), (6, None, 1),
+                              (6, SOME, 1), (7, None, 1), (8, need - 1, 1), (4, 1 << 40, 6)]:
+        args = list(good)
+        args[at] = value
+        assert lib.infmoe_layer_forward_topk(*args) == status, (at, value)
+    assert lib.infmoe_layer_forward_topk(*[0 if i == 4 else v for i, v in enumerate(good)]) == 0
+    layer.terminate()
+
+
+def test_python_refuses_tensors_off_the_device_and_bad_configurations():
+    f = torch.zeros
+    with pytest.raises(ValueError):
+        TopKRouter(8, 2, score="tanh")
+    with pytest.raises(ValueError):
+        TopKRouter(8, 2, bias=f(8))                              # not on a GPU
+    with pytest.raises(capi.InfMoEError):
+        TopKRouter(8, 9)
+    with pytest.raises(capi.InfMoEError):
+        TopKRouter(9, 2, groups=2)
+    with pytest.raises(ValueError):
+        TopKRouter(8, 2).select(f(3, 8))
+    with pytest.raises(ValueError):
+        count_experts(f(6, dtype=torch.int32), 3)
+    with pytest.raises(ValueError):
+        scatter_topk(f(3, 8), f(6, dtype=torch.int32), f(4, dtype=torch.int32), 2)
+    with pytest.raises(ValueError):
+        combine_topk(f(6, 8), f(3, 2))
+    with pytest.raises(ValueError):
+        Adapters(f(2, 4, 8), f(2, 16, 4))
+
+
+def test_reference_choices_by_hand():
+    """The tests' own reference on rows whose answers are plain."""
+    l = np.array([[1.0, 3.0, 2.0, 3.0], [-np.inf, np.nan, 0.0, -np.inf], [-np.inf] * 4])
+    gate, w = topk_ref.select(l, topk_ref.LOWEST["float32"], 2, "softmax")
+    assert gate.tolist() == [[1, 3], [2, -1], [-1, -1]]
+    np.testing.assert_allclose(w, [[0.5, 0.5], [1, 0], [0, 0]])
+    gate, w = topk_ref.select(l[:1], -1e38, 1, "sigmoid", np.array([9.0, 0, 0, 0]), renormalise=False)
+    assert gate.tolist() == [[0]] and abs(w[0, 0] - 1 / (1 + np.exp(-1))) < 1e-15
+    gate, _ = topk_ref.select(np.array([[5.0, -9, 2, 2.5]]), -1e38, 1, "sigmoid", None, 2, 1, 2)
+    assert gate.tolist() == [[3]]                                # 0.993 + 0.0001 against 0.881 + 0.924
