@@ -19,8 +19,8 @@ constexpr int SELECT_WARPS = 8;
 struct SelectArgs {
     const void* logits;      // [T][ld]
     long long T, ld;
-    int E, k, groups, top_groups, group_best, group_size, lanes;
-    int sigmoid, renormalise;
+    int E, k, groups, top_groups, group_best, group_size, lanes, lanes_log2, width_log2;
+    int sigmoid, renormalise, vec;     // vec: a lane's logits are read 16 bytes at a time
     float scale;
     const float* bias;       // [E] or NULL
     int* gate;               // [T][k]
@@ -38,7 +38,7 @@ __device__ __forceinline__ double shfl_xor(double v, int off) { return __shfl_xo
 
 // Expert indices of the k best in lanes 0..k-1, -1 where there are fewer, chosen by scores in 64 bits.
 template <typename T, int V>
-__device__ int select_in_64_bits(const SelectArgs& a, long long t, int lane) {
+__device__ __noinline__ int select_in_64_bits(const SelectArgs& a, long long t, int lane) {
     const T* row = static_cast<const T*>(a.logits) + t * a.ld;
     const int g = lane / a.lanes, first = (lane - g * a.lanes) * V;
     const double none = -INFINITY;
@@ -118,65 +118,328 @@ __device__ int select_in_64_bits(const SelectArgs& a, long long t, int lane) {
     return mine;
 }
 
-// Weights of the chosen experts, whose indices lanes 0..k-1 hold, and the row's answer.  Renormalised weights are computed
-// from the chosen logits alone, relative to the largest, so they do not vanish where all scores do.
-template <typename T, int V>
-__device__ void store_choice(const SelectArgs& a, long long t, int lane, int mine) {
+// The same from scores in 32 bits, as long as these tell all that matters apart; else false, and the choice has to be made in 64.
+//
+// A score becomes a 32-bit key whose order as an unsigned number is that of the scores; an expert that cannot be chosen has the
+// score -inf, the keys up to NONE.  A key's lowest bits give way to the place in the lane, so that sorting keys carries the index
+// along: with V = 8 that moves a score by 2^-20 of itself, no more than what exp and division leave uncertain.  By logits of 16
+// bits nothing moves at all: their FP32 form has 13 bits to spare, which hold the whole index.  A lane sorts its keys (two
+// instructions a comparison), and each round takes the largest of the 32 heads by one redux and moves that lane's list on.  Lists
+// hold four keys; a lane that has more and uses up four of them shows a last one that nothing exceeds, which counts as undecided.
+template <int V>
+struct Keys {
+    static constexpr int PLACE_BITS = V <= 1 ? 0 : V <= 2 ? 1 : V <= 4 ? 2 : V <= 8 ? 3 : V <= 16 ? 4 : 5;
+    static constexpr int DEPTH = V < 4 ? V : 4;
+    static constexpr uint32_t PLACES = (1u << PLACE_BITS) - 1, MORE = 0xffffffffu, NONE = 0x007fffffu;
+};
+
+__device__ __forceinline__ uint32_t key_of(float v) {
+    const uint32_t w = __float_as_uint(v);
+    return w ^ ((uint32_t)((int)w >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t key) {
+    return __uint_as_float(key ^ ((uint32_t)(~(int)key >> 31) | 0x80000000u));
+}
+__device__ __forceinline__ void descending(uint32_t& a, uint32_t& b) {
+    const uint32_t high = max(a, b);
+    b = min(a, b);
+    a = high;
+}
+__device__ __forceinline__ void sort4(uint32_t (&k)[4]) {
+    descending(k[0], k[1]);
+    descending(k[2], k[3]);
+    descending(k[0], k[2]);
+    descending(k[1], k[3]);
+    descending(k[1], k[2]);
+}
+// The largest of n keys (four at most), largest first.
+template <int N>
+__device__ __forceinline__ void largest(const uint32_t* k, uint32_t (&out)[N < 4 ? N : 4]) {
+    if constexpr (N <= 4) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) out[i] = k[i];
+        if constexpr (N == 2) descending(out[0], out[1]);
+        if constexpr (N == 4) sort4(out);
+    } else {
+        uint32_t other[4];
+        largest<N / 2>(k, out);
+        largest<N / 2>(k + N / 2, other);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = max(out[i], other[3 - i]);     // the largest four, rising and falling
+        descending(out[0], out[2]);
+        descending(out[1], out[3]);
+        descending(out[0], out[1]);
+        descending(out[2], out[3]);
+    }
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float reciprocal_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// What experts are chosen by: the logits themselves, or (with a bias, or groups that count with two experts) scores of them.
+enum ChosenBy { LOGITS, SOFTMAX, SIGMOID };
+
+// l[j]: the lane's logits, -inf where there is none to choose; bias[j]: their biases; base: the lane's first expert; found: the
+// warp's place for the rounds' keys and lanes.
+template <typename T, int V, ChosenBy BY>
+__device__ __forceinline__ bool select_in_32_bits(const SelectArgs& a, const float (&l)[V], const float (&bias)[V], int lane, int base,
+                                                  uint2* found, int& mine) {
+    using K = Keys<V>;
+    constexpr bool SCORES = BY != LOGITS;
+    constexpr bool WHOLE = !SCORES && sizeof(T) == 2;               // the key holds the expert's whole place
+    constexpr uint32_t LOW = WHOLE ? 32 * V - 1 : K::PLACES;
+    const uint32_t low0 = WHOLE ? (31 - lane) * V + V - 1 : V - 1;
+    constexpr float LOG2E = 1.4426950408889634f;
+    uint32_t key[V];
+    float uncertain = 0.f;                                          // how far a score may be off, twice, beside what its size leaves
+    if constexpr (SCORES) {
+        float top = 0.f, part = 1.f;
+        if constexpr (BY == SOFTMAX) {
+            top = l[0];
+#pragma unroll
+            for (int j = 1; j < V; ++j) top = fmaxf(top, l[j]);
+            top = warp_max(top);
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < V; ++j) sum += l[j] == top ? 1.f : exp2_fast((l[j] - top) * LOG2E);
+            part = reciprocal_fast(warp_xor_sum(sum));
+        }
+        // Sigmoid: the exponential is off by (2 + 1.2 |l|) 2^-23, which comes to 0.8 of these units, sum, reciprocal and the sum
+        // with the bias to 2.  Softmax: no score exceeds `part`; exponential, sum of up to 1024 of them and reciprocal come to
+        // less than 34 units of it.
+        uncertain = BY == SIGMOID ? 0x1p-20f : part * 0x1p-17f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            float s;
+            if constexpr (BY == SIGMOID)
+                s = reciprocal_fast(1.f + exp2_fast(l[j] * -LOG2E));
+            else
+                s = (l[j] == top ? 1.f : exp2_fast((l[j] - top) * LOG2E)) * part;
+            const float c = l[j] > -INFINITY ? s + bias[j] : -INFINITY;
+            key[j] = (key_of(c) & ~LOW) | (low0 - j);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) key[j] = (key_of(l[j]) & ~LOW) | (low0 - j);
+    }
+    uint32_t head[K::DEPTH];
+    largest<V>(key, head);
+    uint32_t rest = V > K::DEPTH && head[K::DEPTH - 1] > K::NONE ? K::MORE : 0u;
+    constexpr float SPREAD = SCORES ? (float)(1u << K::PLACE_BITS) * 0x1p-21f : 0.f;
+    bool sure = true;
+    if (a.groups > 1) {
+        uint32_t b1 = head[0], b2 = K::DEPTH > 1 ? head[K::DEPTH > 1 ? 1 : 0] : 0u;
+        for (int off = a.lanes >> 1; off >= 1; off >>= 1) {
+            const uint32_t o1 = __shfl_xor_sync(0xffffffffu, b1, off), o2 = __shfl_xor_sync(0xffffffffu, b2, off);
+            b2 = max(min(b1, o1), max(b2, o2));
+            b1 = max(b1, o1);
+        }
+        uint32_t group = b1;
+        float size = SCORES && b1 > K::NONE ? fabsf(value_of(b1 & ~LOW)) : 0.f;     // what the sum's uncertainty goes by
+        if (SCORES && a.group_best == 2 && b2 > K::NONE) {
+            group = key_of(value_of(b1 & ~LOW) + value_of(b2 & ~LOW));
+            size += fabsf(value_of(b2 & ~LOW));
+        }
+        group = b1 > K::NONE ? (group & ~31u) | (31 - (lane >> a.lanes_log2)) : 0u;
+        uint32_t left = group, last = 0u;
+        for (int i = 0; i < a.top_groups; ++i) {
+            last = __reduce_max_sync(0xffffffffu, left);
+            left = left == last ? 0u : left;
+        }
+        const uint32_t next = __reduce_max_sync(0xffffffffu, left);
+        if (next) {
+            if constexpr (SCORES) {
+                size = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(size)));
+                sure = value_of(last & ~31u) - value_of(next & ~31u) > 2.f * uncertain + size * (SPREAD + 0x1p-16f);
+            } else {
+                sure = WHOLE || (last >> 5) != (next >> 5);
+            }
+        }
+        if (group < last || group == 0u) {
+#pragma unroll
+            for (int i = 0; i < K::DEPTH; ++i) head[i] = 0u;
+            rest = 0u;
+        }
+    }
+    // Rounds.  Lanes whose heads are equal move on together: the keys that are lost so are counted, and leave it undecided.
+    int taken = 0, rounds = 0;
+    for (; rounds <= a.k; ++rounds) {
+        const uint32_t top = __reduce_max_sync(0xffffffffu, head[0]);
+        if (top <= K::NONE) break;
+        if (head[0] == top) {
+            found[rounds] = make_uint2(top, (uint32_t)base);
+#pragma unroll
+            for (int d = 0; d + 1 < K::DEPTH; ++d) head[d] = head[d + 1];
+            head[K::DEPTH - 1] = rest;
+            ++taken;
+        }
+    }
+    __syncwarp();
+    const uint2 choice = lane < rounds ? found[lane] : make_uint2(0u, 0u);
+    const uint32_t best = choice.x, after = __shfl_down_sync(0xffffffffu, best, 1);
+    __syncwarp();
+    sure = sure && best != K::MORE;
+    if (!WHOLE && lane < a.k && after) {
+        if constexpr (SCORES) {
+            const float high = value_of(best & ~LOW);
+            sure = sure && high - value_of(after & ~LOW) > uncertain + fabsf(high) * SPREAD;
+        } else {
+            sure = sure && (best & ~LOW) != (after & ~LOW);
+        }
+    }
+    if (__reduce_add_sync(0xffffffffu, (unsigned)taken + (sure ? 0u : 1u << 16)) != (unsigned)rounds) return false;
+    mine = lane < a.k && best ? (int)(choice.y + ((LOW - (best & LOW)) & (V - 1))) : -1;
+    return true;
+}
+
+// Weights of chosen experts, and the answer.  `width` lanes, a power of two, have the experts of one token (-1: none), rank r in
+// the r-th of them.  Renormalised weights are computed from the chosen logits alone, relative to the largest, so they do not vanish
+// where all scores do.
+template <typename T>
+__device__ __forceinline__ void store_choice(const SelectArgs& a, long long t, int r, int mine, int width, bool live) {
     const T* row = static_cast<const T*>(a.logits) + t * a.ld;
-    const float l = mine >= 0 ? to_float(row[mine]) : -INFINITY;
-    const float top = warp_max(l);
+    const float l = live && mine >= 0 ? to_float(row[mine]) : -INFINITY;
     float w = 0.f;
     if (a.renormalise) {
+        float top = l;
+        for (int off = width >> 1; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
         if (a.sigmoid && !(top > 0.f))
             w = mine >= 0 ? expf(l - top) / (1.f + expf(l)) : 0.f;
         else if (a.sigmoid)
             w = mine >= 0 ? 1.f / (1.f + expf(-l)) : 0.f;
         else
             w = mine >= 0 ? (l == top ? 1.f : expf(l - top)) : 0.f;
-        const float sum = warp_xor_sum(w);
+        float sum = w;
+        for (int off = width >> 1; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
         w = mine >= 0 ? w / sum : 0.f;
     } else if (a.sigmoid) {
         w = mine >= 0 ? 1.f / (1.f + expf(-l)) : 0.f;
-    } else {
-        // the sum over all experts of the row
+    } else if (live) {
+        // the sum over all experts of the row, by the token's own lanes
         float all = -INFINITY, sum = 0.f;
-        for (int e = lane; e < a.E; e += 32) {
+        for (int e = r; e < a.E; e += width) {
             const float v = to_float(row[e]);
             all = v > Lowest<T>::value() ? fmaxf(all, v) : all;
         }
-        all = warp_max(all);
-        for (int e = lane; e < a.E; e += 32) {
+        const unsigned lanes = width == 32 ? 0xffffffffu : ((1u << width) - 1u) << ((threadIdx.x & 31) & ~(width - 1));
+        for (int off = width >> 1; off >= 1; off >>= 1) all = fmaxf(all, __shfl_xor_sync(lanes, all, off));
+        for (int e = r; e < a.E; e += width) {
             const float v = to_float(row[e]);
             if (v > Lowest<T>::value()) sum += v == all ? 1.f : expf(v - all);
         }
-        sum = warp_xor_sum(sum);
+        for (int off = width >> 1; off >= 1; off >>= 1) sum += __shfl_xor_sync(lanes, sum, off);
         w = mine >= 0 ? (l == all ? 1.f : expf(l - all)) / sum : 0.f;
     }
-    if (lane < a.k) {
-        a.gate[t * a.k + lane] = mine;
-        a.weight[t * a.k + lane] = w * a.scale;
+    if (live && r < a.k) {
+        a.gate[t * a.k + r] = mine;
+        a.weight[t * a.k + r] = w * a.scale;
+        if (r == 0 && mine < 0 && a.status) atomicOr(a.status, STATUS_NO_EXPERT);
     }
-    if (lane == 0 && mine < 0 && a.status) atomicOr(a.status, STATUS_NO_EXPERT);
 }
 
+// The lane's V logits of a row; -inf for an expert that cannot be chosen, or is not there.
 template <typename T, int V>
-__global__ void __launch_bounds__(SELECT_WARPS * 32) select_topk_kernel(const SelectArgs a) {
+__device__ __forceinline__ void load_logits(const SelectArgs& a, long long t, int first, int count, float (&l)[V]) {
+    const T* row = static_cast<const T*>(a.logits) + t * a.ld + first;
+    constexpr int N = V * sizeof(T) >= 16 ? 16 / (int)sizeof(T) : V;
+    if (a.vec && V * sizeof(T) >= 16) {
+#pragma unroll
+        for (int j = 0; j < V; j += N) {
+            float e[N];
+            load_elems<T, N>(row + j, e);
+#pragma unroll
+            for (int i = 0; i < N; ++i) l[j + i] = e[i];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) l[j] = j < count ? to_float(row[j]) : -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) l[j] = l[j] > Lowest<T>::value() ? l[j] : -INFINITY;    // NaN too
+}
+
+// A warp per token, tokens a grid apart, 32 to a warp before the block meets.  As many tokens as fit into the lanes (four with 5 to
+// 8 experts each) then get their weights together: by token that took 10 of 45 us (65536 tokens, 8 of 256 experts).  Tokens
+// that 32 bits leave undecided wait until the block's are done; in the loop itself that choice cost every token its registers, 20 us.
+template <typename T, int V, ChosenBy BY>
+__global__ void __launch_bounds__(SELECT_WARPS * 32, V <= 8 ? 4 : V <= 16 ? 3 : 2) select_topk_kernel(const __grid_constant__ SelectArgs a) {
+    __shared__ uint2 s_found[SELECT_WARPS][17];
+    __shared__ int s_choice[SELECT_WARPS][32];
+    __shared__ int s_open[SELECT_WARPS * 32], s_open_count;         // undecided tokens: warp and turn
     pdl_trigger();
     pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const long long t = (long long)blockIdx.x * SELECT_WARPS + (threadIdx.x >> 5);
-    if (t >= a.T) return;
-    const int mine = select_in_64_bits<T, V>(a, t, lane);
-    store_choice<T, V>(a, t, lane, mine);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int g = lane >> a.lanes_log2, place = (lane & (a.lanes - 1)) * V;
+    const int first = g * a.group_size + place, count = g < a.groups ? a.group_size - place : 0;    // its experts
+    float bias[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        bias[j] = BY != LOGITS && a.bias && j < count ? a.bias[first + j] : 0.f;
+        if (bias[j] != bias[j]) bias[j] = -INFINITY;
+    }
+    const long long step = (long long)gridDim.x * SELECT_WARPS;
+    const int width = 1 << a.width_log2, batch = 32 >> a.width_log2, r = lane & (width - 1);
+    for (long long t0 = (long long)blockIdx.x * SELECT_WARPS; t0 < a.T; t0 += 32 * step) {      // the block's next 32 turns
+        if (threadIdx.x == 0) s_open_count = 0;
+        __syncthreads();
+        for (int turn = 0; turn < 32 && t0 + warp + turn * step < a.T; turn += batch) {
+            s_choice[warp][lane] = -2;
+            __syncwarp();
+            for (int i = 0; i < batch; ++i) {
+                const long long t = t0 + warp + (turn + i) * step;
+                if (t >= a.T) break;
+                float l[V];
+                load_logits<T, V>(a, t, first, count, l);
+                int mine = -1;
+                if (a.k <= 16 && select_in_32_bits<T, V, BY>(a, l, bias, lane, first, s_found[warp], mine)) {
+                    if (lane < width) s_choice[warp][i * width + lane] = mine;
+                } else if (lane == 0) {
+                    s_open[atomicAdd(&s_open_count, 1)] = warp * 32 + turn + i;
+                }
+            }
+            __syncwarp();
+            const int mine = s_choice[warp][lane];
+            const long long t = t0 + warp + (turn + (lane >> a.width_log2)) * step;
+            store_choice<T>(a, min(t, a.T - 1), r, mine, width, mine != -2);
+            __syncwarp();
+        }
+        __syncthreads();
+        const int open = s_open_count;
+        for (int i = warp; i < open; i += SELECT_WARPS) {
+            const long long t = t0 + (s_open[i] >> 5) + (s_open[i] & 31) * step;
+            const int mine = select_in_64_bits<T, V>(a, t, lane);
+            store_choice<T>(a, t, lane, mine, 32, true);
+        }
+        __syncthreads();
+    }
 }
 
-template <typename T, int V>
-int launch_select(const SelectArgs& a, cudaStream_t stream) {
-    const long long grid = (a.T + SELECT_WARPS - 1) / SELECT_WARPS;
-    INFMOE_CUDA_TRY(launch_chained(select_topk_kernel<T, V>, (unsigned)grid, SELECT_WARPS * 32, 0, 1, stream, a));
+template <typename T, int V, ChosenBy BY>
+int launch_select_kernel(const SelectArgs& a, cudaStream_t stream) {
+    const long long blocks = (a.T + SELECT_WARPS - 1) / SELECT_WARPS, most = 148 * (V <= 8 ? 4 : V <= 16 ? 3 : 2);   // as many as run at once
+    INFMOE_CUDA_TRY(launch_chained(select_topk_kernel<T, V, BY>, (unsigned)(blocks < most ? blocks : most), SELECT_WARPS * 32, 0, 1,
+                                   stream, a));
     note_launch();
     INFMOE_CUDA_TRY(cudaGetLastError());
     return INFMOE_OK;
+}
+
+template <typename T, int V>
+int launch_select(SelectArgs a, cudaStream_t stream) {
+    constexpr int bytes = V * (int)sizeof(T) < 16 ? V * (int)sizeof(T) : 16;
+    a.vec = a.group_size == a.lanes * V && a.groups * a.lanes == 32 && (uintptr_t)a.logits % bytes == 0 &&
+            a.ld * (long long)sizeof(T) % bytes == 0;
+    if (!a.bias && (a.groups == 1 || a.group_best == 1)) return launch_select_kernel<T, V, LOGITS>(a, stream);
+    if (a.sigmoid) return launch_select_kernel<T, V, SIGMOID>(a, stream);
+    return launch_select_kernel<T, V, SOFTMAX>(a, stream);
 }
 
 template <typename T>
@@ -368,6 +631,9 @@ int infmoe_expert_select_topk(const infmoe_topk_config* cfg, int64_t T, const vo
     a.group_best = cfg->group_best;
     a.group_size = size;
     a.lanes = lanes;
+    a.lanes_log2 = 0;
+    while ((1 << a.lanes_log2) < lanes) ++a.lanes_log2;
+    while ((1 << a.width_log2) < k) ++a.width_log2;      // lanes that hold the experts of a token
     a.sigmoid = cfg->score == INFMOE_SCORE_SIGMOID;
     a.renormalise = cfg->renormalise != 0;
     a.scale = cfg->scale;
