@@ -12,7 +12,7 @@ from __future__ import annotations
 import ctypes
 
 from . import capi
-from .topk import check_array, dtype_code, launch, rows_of
+from .topk import binding, check_array, launch
 
 __all__ = ["Adapters", "AdapterPlan"]
 
@@ -56,12 +56,16 @@ class Adapters:
         if rank is not None:
             check_array(rank, (n,), torch.int32, a.device, "rank")
         self._tensors = (a, b, scale, rank)
-        self._set = capi.AdapterSet(n, r, d_in, self.d_out, dtype_code(a), a.data_ptr(), b.data_ptr(),
+        codes = {torch.float32: capi.DTYPE_F32, torch.float16: capi.DTYPE_F16, torch.bfloat16: capi.DTYPE_BF16}
+        if a.dtype not in codes:
+            raise ValueError(f"adapters of {a.dtype} are not supported: use float32, float16 or bfloat16")
+        self._set = capi.AdapterSet(n, r, d_in, self.d_out, codes[a.dtype], a.data_ptr(), b.data_ptr(),
                                     scale.data_ptr() if scale is not None else None,
                                     rank.data_ptr() if rank is not None else None)
-        self._set_ref = ctypes.byref(self._set)
+        self._apply = binding().apply_adapters
         # what a set can be refused for, now and not at the first call: no tokens, no device work
-        capi.check(capi.lib().infmoe_adapter_apply(self._set_ref, 0, None, d_in, None, self.d_out, None, self.d_out, None, None))
+        capi.check(capi.lib().infmoe_adapter_apply(ctypes.byref(self._set), 0, None, d_in, None, self.d_out, None, self.d_out,
+                                                    None, None))
 
     def plan(self, adapter_of_token) -> AdapterPlan:
         """adapter_of_token: int32 CUDA tensor, one index per token; an index outside [0, n) means none."""
@@ -69,22 +73,4 @@ class Adapters:
 
     def apply(self, x, y, plan: AdapterPlan, out=None):
         """x [..., d_in], y [..., d_out] -> y plus each row's adapter of x.  out may be y (in place), not x."""
-        import torch
-
-        T, ldx = rows_of(x, self.d_in, "x")
-        Ty, ldy = rows_of(y, self.d_out, "y")
-        if x.dtype != self.dtype or y.dtype != self.dtype or x.device != self.device or y.device != self.device:
-            raise ValueError(f"x and y must be {str(self.dtype)[6:]} tensors on {self.device}, like the adapters")
-        if T != Ty or T != plan.tokens or plan.adapter_count != self.adapter_count or plan.device != self.device:
-            raise ValueError(f"x has {T} rows, y {Ty}; the plan is for {plan.tokens} rows and {plan.adapter_count} adapters on "
-                             f"{plan.device}, the set has {self.adapter_count} on {self.device}")
-        if out is None:
-            out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-            ldo = self.d_out
-        else:
-            To, ldo = rows_of(out, self.d_out, "out")
-            if To != T or out.shape != y.shape or out.dtype != self.dtype or out.device != self.device:
-                raise ValueError("out must be a tensor like y")
-        launch(x.get_device(), "infmoe_adapter_apply", self._set_ref, T, x.data_ptr(), ldx, y.data_ptr(), ldy, out.data_ptr(),
-               ldo, plan.buffer.data_ptr())
-        return out
+        return self._apply(self._set, self._tensors[0], x, y, plan.buffer, plan.tokens, plan.adapter_count, out)

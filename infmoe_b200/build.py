@@ -1,15 +1,17 @@
 """Builds the native libraries in-tree with nvcc for sm_100a.
 
-    python -m infmoe_b200.build          # libinfmoe_b200.so (+ libtrtmoelayer.so)
+    python -m infmoe_b200.build          # libinfmoe_b200.so (+ libtrtmoelayer.so, _binding.so)
 
 nvcc cross-compiles without a GPU.  Objects are cached under infmoe_b200/build/
 and rebuilt when a source or header is newer.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -18,6 +20,7 @@ CSRC = os.path.join(PKG, "csrc")
 OBJ = os.path.join(PKG, "build")
 LIB = os.path.join(PKG, "libinfmoe_b200.so")
 PLUGIN_LIB = os.path.join(PKG, "libtrtmoelayer.so")
+BINDING = os.path.join(PKG, "_binding.so")      # calls on torch tensors (csrc/binding.cc)
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-fvisibility=hidden",
@@ -77,6 +80,27 @@ def _link(nvcc: str, objs, out: str, extra, verbose: bool) -> None:
             raise RuntimeError(f"link failed for {out}:\n{r.stdout}\n{r.stderr}")
 
 
+def _build_binding(verbose: bool) -> None:
+    """The extension module, compiled against the installed torch's headers."""
+    src = os.path.join(CSRC, "binding.cc")
+    if not _stale(BINDING, [src, os.path.join(ROOT, "include", "infmoe_c.h")]):
+        return
+    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
+    cuda = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include")
+    includes = [sysconfig.get_paths()["include"], os.path.join(torch, "include"),
+                os.path.join(torch, "include", "torch", "csrc", "api", "include"), cuda]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared", "-I", os.path.join(ROOT, "include")]
+    cmd += [f for d in includes for f in ("-isystem", d)] + [src, "-o", BINDING, "-L", PKG, "-linfmoe_b200", "-L",
+                                                             os.path.join(torch, "lib")]
+    cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN",
+            "-Wl,-rpath," + os.path.join(torch, "lib")]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for binding.cc:\n{r.stdout}\n{r.stderr}")
+
+
 def build(verbose: bool = False) -> str:
     nvcc = _nvcc()
     os.makedirs(OBJ, exist_ok=True)
@@ -87,6 +111,7 @@ def build(verbose: bool = False) -> str:
     _link(nvcc, core, LIB, ["-lz", "-ldl"], verbose)
     if plug:
         _link(nvcc, plug, PLUGIN_LIB, ["-L", PKG, "-linfmoe_b200", "-Xlinker", "-rpath,$ORIGIN"], verbose)
+    _build_binding(verbose)
     return LIB
 
 

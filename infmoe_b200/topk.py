@@ -14,25 +14,25 @@ All functions work on torch's current stream of the tensors' device, and allocat
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Tuple
 
 from . import capi
 
 __all__ = ["TopKRouter", "count_experts", "scatter_topk", "combine_topk"]
 
-_DTYPES = {}
+
+def binding():
+    """The extension module that checks tensors, makes outputs and calls the library (csrc/binding.cc)."""
+    global _binding
+    if _binding is None:
+        import torch  # noqa: F401  its libraries come before the module's
+
+        from . import _binding as module
+
+        _binding = module
+    return _binding
 
 
-def dtype_code(t) -> int:
-    """infmoe_dtype of a tensor; ValueError for types the library does not take."""
-    if not _DTYPES:
-        import torch
-
-        _DTYPES.update({torch.float32: capi.DTYPE_F32, torch.float16: capi.DTYPE_F16, torch.bfloat16: capi.DTYPE_BF16})
-    code = _DTYPES.get(t.dtype)
-    if code is None:
-        raise ValueError(f"tensors of {t.dtype} are not supported: use float32, float16 or bfloat16")
-    return code
+_binding = None
 
 
 def launch(device: int, name: str, *args) -> None:
@@ -47,21 +47,6 @@ def launch(device: int, name: str, *args) -> None:
     else:
         with torch.cuda.device(device):
             capi.check(fn(*args, _current_stream(torch, device)))
-
-
-def rows_of(t, width: int, what: str) -> Tuple[int, int]:
-    """(rows, row stride) of a CUDA tensor [..., width]: rows apart by any stride for [T, width], contiguous otherwise."""
-    if not t.is_cuda or t.dim() < 1 or t.shape[-1] != width or (width > 1 and t.stride(-1) != 1):
-        raise ValueError(f"{what} must be a CUDA tensor [..., {width}] with consecutive elements in a row")
-    rows = t.numel() // width
-    if t.dim() == 2 and rows > 1:
-        ld = t.stride(0)
-        if ld < width:
-            raise ValueError(f"the rows of {what} overlap (stride {ld})")
-        return rows, ld
-    if t.dim() > 2 and not t.is_contiguous():
-        raise ValueError(f"{what} must be contiguous (or two-dimensional)")
-    return rows, width
 
 
 def check_array(t, shape, dtype, device, what: str) -> None:
@@ -94,9 +79,9 @@ class TopKRouter:
         self.expert_count, self.top_k, self.bias = int(expert_count), int(top_k), bias
         self._cfg = capi.TopKConfig(expert_count, top_k, capi.SCORES[score], groups, top_groups, group_best, int(renormalise),
                                     scale)
-        self._cfg_ref = ctypes.byref(self._cfg)
+        self._select = binding().select_topk
         # what a configuration can be refused for, now and not at the first call: no tokens, no device work
-        capi.check(capi.lib().infmoe_expert_select_topk(self._cfg_ref, 0, None, capi.DTYPE_F32, expert_count, None, None, None,
+        capi.check(capi.lib().infmoe_expert_select_topk(ctypes.byref(self._cfg), 0, None, capi.DTYPE_F32, expert_count, None, None, None,
                                                         None, None))
 
     def select(self, logits, gate=None, weight=None, status=None):
@@ -104,27 +89,7 @@ class TopKRouter:
 
         Experts with a logit of NaN or of the type's lowest value or less (-inf) are not chosen; places that stay empty hold
         gate -1 and weight 0.  status (int32 [1], may be None): bit 0 is set when a token has no expert at all."""
-        import torch
-
-        T, ld = rows_of(logits, self.expert_count, "logits")
-        code, device, k = dtype_code(logits), logits.device, self.top_k
-        if self.bias is not None and self.bias.device != device:
-            raise ValueError(f"logits are on {device}, the router's bias on {self.bias.device}")
-        shape = (*logits.shape[:-1], k)
-        if gate is None:
-            gate = torch.empty(shape, dtype=torch.int32, device=device)
-        else:
-            check_array(gate, shape, torch.int32, device, "gate")
-        if weight is None:
-            weight = torch.empty(shape, dtype=torch.float32, device=device)
-        else:
-            check_array(weight, shape, torch.float32, device, "weight")
-        if status is not None:
-            check_array(status, (1,), torch.int32, device, "status")
-        launch(logits.get_device(), "infmoe_expert_select_topk", self._cfg_ref, T, logits.data_ptr(), code, ld,
-               self.bias.data_ptr() if self.bias is not None else None, gate.data_ptr(), weight.data_ptr(),
-               status.data_ptr() if status is not None else None)
-        return gate, weight
+        return self._select(self._cfg, logits, self.bias, gate, weight, status)
 
 
 def count_experts(gate, expert_count: int, status=None):
@@ -149,26 +114,7 @@ def scatter_topk(x, pos, offset, top_k: int, out=None, row_of=None):
     """x [..., D] -> (rows in expert order [T * top_k, D], row of every slot [T, top_k], -1 for slots without an expert).
 
     pos and offset are count_experts' of the slots; rows behind the last expert's are left as they are in `out`."""
-    import torch
-
-    D = x.shape[-1]
-    T, ld = rows_of(x, D, "x")
-    slots, device = T * top_k, x.device
-    check_array(pos, (slots,), torch.int32, device, "pos")
-    if offset.dim() != 1 or offset.numel() < 1:
-        raise ValueError("offset must hold expert_count + 1 row numbers")
-    check_array(offset, offset.shape, torch.int32, device, "offset")
-    if out is None:
-        out = torch.empty((slots, D), dtype=x.dtype, device=device)
-    else:
-        check_array(out, (slots, D), x.dtype, device, "out")
-    if row_of is None:
-        row_of = torch.empty((T, top_k), dtype=torch.int32, device=device)
-    else:
-        check_array(row_of, (T, top_k), torch.int32, device, "row_of")
-    launch(x.get_device(), "infmoe_expert_scatter_topk", T, top_k, D, dtype_code(x), x.data_ptr(), ld, pos.data_ptr(),
-           offset.data_ptr() + 4 * (offset.numel() - 1), out.data_ptr(), row_of.data_ptr())
-    return out, row_of
+    return binding().scatter_topk(x, pos, offset, top_k, out, row_of)
 
 
 def combine_topk(rows, weight, row_of=None, gate=None, residual=None, out=None):
@@ -177,28 +123,4 @@ def combine_topk(rows, weight, row_of=None, gate=None, residual=None, out=None):
     rows [n, D]; weight float32 [..., top_k]; row_of int32 like weight (None: slot (t, s) is row t * top_k + s); gate int32
     like weight or None: slots with a negative gate are left out, like slots whose row lies outside [0, n).  residual, out:
     [..., D] like weight's leading dimensions; out may be residual."""
-    import torch
-
-    device = rows.device
-    if rows.dim() != 2 or not rows.is_cuda or not rows.is_contiguous():
-        raise ValueError("rows must be a contiguous CUDA tensor [n, D]")
-    n, D = rows.shape
-    if weight.dim() < 1:
-        raise ValueError("weight must be [..., top_k]")
-    k = weight.shape[-1]
-    check_array(weight, weight.shape, torch.float32, device, "weight")
-    T = weight.numel() // k if k else 0
-    shape = (*weight.shape[:-1], D)
-    for t, what in ((row_of, "row_of"), (gate, "gate")):
-        if t is not None:
-            check_array(t, weight.shape, torch.int32, device, what)
-    if residual is not None:
-        check_array(residual, shape, rows.dtype, device, "residual")
-    if out is None:
-        out = torch.empty(shape, dtype=rows.dtype, device=device)
-    else:
-        check_array(out, shape, rows.dtype, device, "out")
-    launch(rows.get_device(), "infmoe_expert_combine_topk", T, k, D, dtype_code(rows), rows.data_ptr(), n, weight.data_ptr(),
-           gate.data_ptr() if gate is not None else None, row_of.data_ptr() if row_of is not None else None,
-           residual.data_ptr() if residual is not None else None, out.data_ptr())
-    return out
+    return binding().combine_topk(rows, weight, row_of, gate, residual, out)
