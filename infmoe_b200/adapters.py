@@ -63,14 +63,15 @@ class Adapters:
                                     scale.data_ptr() if scale is not None else None,
                                     rank.data_ptr() if rank is not None else None)
         self._apply = binding().apply_adapters
-        # what a set can be refused for, now and not at the first call: no tokens, no device work
-        capi.check(capi.lib().infmoe_adapter_apply(ctypes.byref(self._set), 0, None, d_in, None, self.d_out, None, self.d_out,
-                                                    None, None))
+        # what a set can be refused for, now and not at the first call
+        capi.check(capi.lib().infmoe_adapter_workspace_bytes(ctypes.byref(self._set), 0, ctypes.byref(ctypes.c_size_t())))
 
     def plan(self, adapter_of_token) -> AdapterPlan:
         """adapter_of_token: int32 CUDA tensor, one index per token; an index outside [0, n) means none."""
         return AdapterPlan(adapter_of_token, self.adapter_count)
 
-    def apply(self, x, y, plan: AdapterPlan, out=None):
-        """x [..., d_in], y [..., d_out] -> y plus each row's adapter of x.  out may be y (in place), not x."""
-        return self._apply(self._set, self._tensors[0], x, y, plan.buffer, plan.tokens, plan.adapter_count, out)
+    def apply(self, x, y, plan: AdapterPlan, out=None, status=None):
+        """x [..., d_in], y [..., d_out] -> y plus each row's adapter of x.  out may be y (in place), not x.
+
+        status (int32 [1], may be None): bit 2 is set when a bounded wait inside a kernel ran out."""
+        return self._apply(self._set, self._tensors[0], x, y, plan.buffer, plan.tokens, plan.adapter_count, out, status)

@@ -177,7 +177,8 @@ SIGNATURES = {
     "infmoe_expert_combine_topk": [_i64, _i32, _i32, _i32, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp],
     "infmoe_adapter_plan_bytes": [_i64, _i32, ctypes.POINTER(_sz)],
     "infmoe_adapter_plan": [_i64, _i32, _vp, _vp, _sz, _vp],
-    "infmoe_adapter_apply": [ctypes.POINTER(AdapterSet), _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp],
+    "infmoe_adapter_workspace_bytes": [ctypes.POINTER(AdapterSet), _i64, ctypes.POINTER(_sz)],
+    "infmoe_adapter_apply": [ctypes.POINTER(AdapterSet), _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _sz, _vp, _vp],
     "infmoe_register_sublayer": [ctypes.c_char_p, ctypes.POINTER(SublayerVtable)],
     "infmoe_ep_unique_id": [_vp],
     "infmoe_ep_create": [ctypes.POINTER(EpConfig), ctypes.POINTER(_vp)],

@@ -210,7 +210,7 @@ PyObject* combine_topk(PyObject* const* a) {
     return wrap(out);
 }
 
-// (set, a, x, y, plan buffer, plan tokens, plan adapters, out) -> out
+// (set, a, x, y, plan buffer, plan tokens, plan adapters, out, status) -> out
 PyObject* apply_adapters(PyObject* const* a) {
     const Held<infmoe_adapter_set> set(a[0]);
     const at::Tensor &weights = tensor(a[1], "a"), &x = tensor(a[2], "x"), &y = tensor(a[3], "y"), &plan = tensor(a[4], "plan");
@@ -224,6 +224,8 @@ PyObject* apply_adapters(PyObject* const* a) {
     if (rx.count != ry.count || rx.count != tokens || adapters != set->adapter_count || plan.device() != device)
         refuse("x has %lld rows, y %lld; the plan is for %lld rows and %lld adapters on %s, the set has %d on %s", (long long)rx.count,
                (long long)ry.count, tokens, adapters, plan.device().str().c_str(), set->adapter_count, device.str().c_str());
+    const at::Tensor status = optional(a[8], "status");
+    if (status.defined()) check_array(status, {1}, at::kInt, device, "status");
     at::Tensor out;
     int64_t ldo = set->d_out;
     if (a[7] == Py_None) {
@@ -234,8 +236,11 @@ PyObject* apply_adapters(PyObject* const* a) {
         if (out.sizes() != y.sizes() || out.scalar_type() != type || out.device() != device) refuse("out must be a tensor like y");
     }
     const On on(x);
+    size_t bytes = 0;
+    check(infmoe_adapter_workspace_bytes(set.get(), rx.count, &bytes));
+    const at::Tensor workspace = at::detail::empty_cuda({(int64_t)bytes}, at::kByte, device, std::nullopt);
     check(infmoe_adapter_apply(set.get(), rx.count, x.data_ptr(), rx.ld, y.data_ptr(), ry.ld, out.data_ptr(), ldo, plan.data_ptr(),
-                               on.stream));
+                               workspace.data_ptr(), bytes, (int32_t*)data(status), on.stream));
     return wrap(out);
 }
 
@@ -243,7 +248,7 @@ PyMethodDef methods[] = {
     {"select_topk", (PyCFunction)(void (*)())Entry<select_topk>::call<6>, METH_FASTCALL, nullptr},
     {"scatter_topk", (PyCFunction)(void (*)())Entry<scatter_topk>::call<6>, METH_FASTCALL, nullptr},
     {"combine_topk", (PyCFunction)(void (*)())Entry<combine_topk>::call<6>, METH_FASTCALL, nullptr},
-    {"apply_adapters", (PyCFunction)(void (*)())Entry<apply_adapters>::call<8>, METH_FASTCALL, nullptr},
+    {"apply_adapters", (PyCFunction)(void (*)())Entry<apply_adapters>::call<9>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -235,3 +235,124 @@ def test_layer_with_adapters_and_captured():
     assert torch.equal(out, layer.forward(x, adapters=adapters, plan=adapters.plan(at)))
     del g
     layer.terminate()
+
+
+# Many tokens to an adapter and wide ranks in 16 bits take the kernels on tiles of 128 rows: from 2048 tokens on (rank over 32) or 4096
+# (over 16), 32 tokens to an adapter; both sides of these lines, tiles that end anywhere, rows of every alignment.
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("T,n,r,d_in,d_out,requests", [
+    (2047, 1, 64, 64, 64, 1), (2048, 1, 64, 256, 512, 1), (2048, 64, 33, 136, 72, 64), (2048, 65, 33, 136, 72, 64),
+    (2100, 3, 40, 130, 76, 9), (2500, 60, 100, 520, 264, 70), (4095, 2, 32, 64, 200, 5), (4096, 2, 32, 64, 200, 5),
+    (4096, 2, 17, 72, 1000, 5), (4096, 2, 16, 72, 1000, 5), (4500, 7, 128, 1000, 130, 40), (2300, 2, 64, 63, 65, 5),
+    (2049, 1, 128, 8, 4100, 2), (3000, 4, 65, 2056, 64, 2900)])
+def test_whole_numbers_of_many_tokens(T, n, r, d_in, d_out, requests, dtype):
+    test_whole_numbers(T, n, r, d_in, d_out, requests, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_many_tokens_rows_apart_and_unaligned(dtype):
+    rng = np.random.default_rng(14)
+    t = TYPES[dtype]
+    T, n, r, d_in, d_out = 2200, 3, 48, 96, 160
+    xs, ys = whole(rng, (T, d_in + 9), 2, t), whole(rng, (T, d_out + 9), 50, t)
+    a, b = whole(rng, (n, r, d_in), 2, t), whole(rng, (n, d_out, r), 1, t)
+    at = owners(rng, T, n, 20)
+    adapters = Adapters(a, b)
+    plan = adapters.plan(torch.from_numpy(at).cuda())
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for i, j in ((0, 0), (1, 0), (0, 3), (8, 8)):
+        x, y = xs[:, i:i + d_in], ys[:, j:j + d_out]
+        want = reference(x, y, a, b, 1, None, at)
+        outs = torch.full((T + 2, d_out + 5), 9.0, device="cuda", dtype=t)
+        adapters.apply(x, y, plan, out=outs[:T, 2:2 + d_out], status=status)
+        check_exact(outs[:T, 2:2 + d_out], want, t)
+        assert (outs[T:] == 9).all() and (outs[:, :2] == 9).all() and (outs[:, 2 + d_out:] == 9).all()
+        keep = ys.clone()
+        adapters.apply(x, keep[:, j:j + d_out], plan, out=keep[:, j:j + d_out])
+        check_exact(keep[:, j:j + d_out], want, t)
+        assert torch.equal(keep[:, :j], ys[:, :j]) and torch.equal(keep[:, j + d_out:], ys[:, j + d_out:])
+    assert int(status) == 0
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_many_tokens_nobody_elses_numbers(dtype):
+    """test_nobody_elses_numbers on tiles of 128 rows."""
+    rng = np.random.default_rng(19)
+    t = TYPES[dtype]
+    T, n, r, d_in, d_out = 2400, 4, 64, 200, 136
+    x, y = whole(rng, (T, d_in), 2, t), whole(rng, (T, d_out), 50, t)
+    a, b = whole(rng, (n, r, d_in), 2, t), whole(rng, (n, d_out, r), 1, t)
+    at = np.array([0, 1, -1, 3] * 600, np.int32)
+    rank = torch.tensor([64, 21, 64, 37], dtype=torch.int32, device="cuda")
+    want = reference(x, y, a, b, 1, rank, at)
+    a[2], b[2] = np.nan, np.inf                                     # nobody's adapter
+    a[1, 21:], b[1, :, 21:] = np.nan, np.nan                        # past its rank
+    a[3, 37:], b[3, :, 37:] = np.inf, -np.inf
+    x[2], x[6], x[10] = np.nan, np.inf, torch.finfo(t).max          # of tokens without an adapter
+    y[2], y[6] = np.nan, -np.inf
+    x[4, 3] = np.nan                                                # a token of adapter 0
+    adapters = Adapters(a, b, rank=rank)
+    got = adapters.apply(x, y, adapters.plan(torch.from_numpy(at).cuda()))
+    rest = np.setdiff1d(np.arange(T), [2, 4, 6])
+    check_exact(got[rest], want[rest], t)
+    assert torch.isnan(got[2]).all() and (got[6] == -np.inf).all() and torch.isnan(got[4]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_many_tokens_against_64_bits(dtype):
+    test_against_64_bits(2200, 3, 64, 1000, 300, dtype)
+    test_against_64_bits(2200, 3, 128, 4096, 72, dtype)
+
+
+def test_many_tokens_on_two_streams_with_one_plan():
+    """A plan serves calls that run at once; each has its workspace."""
+    rng = np.random.default_rng(23)
+    t = torch.bfloat16
+    T, n, r, d = 3000, 3, 64, 512
+    at = owners(rng, T, n, 12)
+    sets = [Adapters(whole(rng, (n, r, d), 2, t), whole(rng, (n, d, r), 1, t)) for _ in range(2)]
+    xs, ys = [whole(rng, (T, d), 2, t) for _ in range(2)], [whole(rng, (T, d), 50, t) for _ in range(2)]
+    plan = sets[0].plan(torch.from_numpy(at).cuda())
+    want = [s.apply(x, y, plan).clone() for s, x, y in zip(sets, xs, ys)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(sets[i].apply(xs[i], ys[i], plan))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+def test_many_tokens_captured_behind_a_layer():
+    """The layer's last kernel, then the adapters' kernels, which start early, twice over in one graph."""
+    from tests.test_gpu_topk import small_layer
+
+    layer, _, _ = small_layer(4, 64, 128, on_device=True)
+    rng = np.random.default_rng(29)
+    f = lambda *s: torch.from_numpy(rng.standard_normal(s).astype(np.float32) * 0.1).cuda()  # noqa: E731
+    x = f(2500, 64)
+    sets = [Adapters(f(2, 40, 64).bfloat16(), f(2, 64, 40).bfloat16()) for _ in range(2)]
+    at = torch.from_numpy(owners(rng, 2500, 2, 6)).cuda()
+
+    def step():
+        h, plan = layer.forward(x).bfloat16(), sets[0].plan(at)
+        for s in sets:
+            h = s.apply(h, h, plan)
+        return h
+
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for seed in (1, 2):
+        x.copy_(torch.from_numpy(np.random.default_rng(seed).standard_normal((2500, 64)).astype(np.float32)))
+        at.copy_(torch.from_numpy(owners(np.random.default_rng(seed), 2500, 2, 9)).cuda())
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, step())
+    del g
+    layer.terminate()

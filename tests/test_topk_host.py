@@ -54,15 +54,15 @@ def test_combine_refuses_bad_arguments(at, value, status):
     assert capi.lib().infmoe_expert_combine_topk(*args) == status
 
 
-def _apply(T=4, x=SOME, ldx=32, y=2 * SOME, ldy=48, out=3 * SOME, ldo=48, plan=4 * SOME, **kw):
+def _apply(T=4, x=SOME, ldx=32, y=2 * SOME, ldy=48, out=3 * SOME, ldo=48, plan=4 * SOME, ws=5 * SOME, ws_bytes=1 << 20, **kw):
     s = capi.AdapterSet(**{**dict(adapter_count=3, rank=8, d_in=32, d_out=48, dtype=2, d_a=SOME, d_b=SOME), **kw})
-    return capi.lib().infmoe_adapter_apply(ctypes.byref(s), T, x, ldx, y, ldy, out, ldo, plan, None)
+    return capi.lib().infmoe_adapter_apply(ctypes.byref(s), T, x, ldx, y, ldy, out, ldo, plan, ws, ws_bytes, None, None)
 
 
 @pytest.mark.parametrize("bad", [dict(T=-1), dict(x=None), dict(y=None), dict(out=None), dict(plan=None), dict(plan=8),
                                  dict(ldx=31), dict(ldy=47), dict(ldo=47), dict(out=SOME), dict(out=2 * SOME, ldo=64),
                                  dict(adapter_count=0), dict(rank=0), dict(d_in=0), dict(d_out=-1), dict(dtype=5),
-                                 dict(d_a=None), dict(d_b=None)], ids=str)
+                                 dict(d_a=None), dict(d_b=None), dict(ws=None), dict(ws=8), dict(ws_bytes=100)], ids=str)
 def test_apply_refuses_bad_arguments(bad):
     assert _apply(**bad) == 1 and "adapter_apply" in capi.last_error()
 
