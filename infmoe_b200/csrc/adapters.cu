@@ -182,12 +182,12 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// An FP32 value as two of 11 significant bits, the second of which the tensor core cuts off behind the eleventh: 2^-21 of the
-// value is left out at most.  An infinity has no second part.
+// An FP32 value as two of 11 significant bits: cut off behind the eleventh, and what is left of it, rounded.  2^-22 of the value is
+// left out at most.  An infinity has no second part.
 __device__ __forceinline__ void split_tf32(const uint32_t v, uint32_t& hi, uint32_t& lo) {
     hi = v & 0xffffe000u;
     const float rest = __fsub_rn(__uint_as_float(v), __uint_as_float(hi));      // NaN for NaN
-    lo = (v & 0x7fffffffu) == 0x7f800000u ? 0u : __float_as_uint(rest);
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"((v & 0x7fffffffu) == 0x7f800000u ? 0.f : rest));
 }
 
 // What is left of v after its rounding to T (0 where that is no finite value).

@@ -12,6 +12,7 @@ namespace infmoe {
 namespace {
 
 constexpr int SELECT_WARPS = 8;
+constexpr int MAX_FAST_K = 16, MAX_ROUNDS = 18;   // experts of a token that 32 bits can choose; from there on lists of four keys run out too often
 
 // Experts are laid out over the lanes of a warp so that a group's experts sit on lanes of their own: groups are padded to a
 // power of two, group g has `lanes` = 32 / padded lanes, and each of these holds V consecutive experts of the group.  So
@@ -102,13 +103,17 @@ __device__ __noinline__ int select_in_64_bits(const SelectArgs& a, long long t, 
         double best = none;
 #pragma unroll
         for (int j = 0; j < V; ++j) best = fmax(best, c[j]);
-        double top = best;
-        for (int off = 16; off >= 1; off >>= 1) top = fmax(top, shfl_xor(top, off));
-        if (!(top > none)) break;
-        const int owner = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
+        // the largest of the lanes': numbers of 64 bits in the scores' order, upper halves first
+        const long long w = __double_as_longlong(best + 0.0);       // -0 is 0
+        const unsigned long long key = (unsigned long long)w ^ ((unsigned long long)(w >> 63) | 0x8000000000000000ull);
+        const unsigned high = __reduce_max_sync(0xffffffffu, (unsigned)(key >> 32));
+        const bool in = (unsigned)(key >> 32) == high;
+        const unsigned low = __reduce_max_sync(0xffffffffu, in ? (unsigned)key : 0u);
+        const int owner = __ffs(__ballot_sync(0xffffffffu, in && (unsigned)key == low)) - 1;
+        if (high == 0x000fffffu) break;                             // -inf
         int place = 0;
 #pragma unroll
-        for (int j = V - 1; j >= 0; --j) place = c[j] == top ? j : place;
+        for (int j = V - 1; j >= 0; --j) place = c[j] == best ? j : place;
 #pragma unroll
         for (int j = 0; j < V; ++j)
             if (lane == owner && j == place) c[j] = none;
@@ -125,11 +130,12 @@ __device__ __noinline__ int select_in_64_bits(const SelectArgs& a, long long t, 
 // along: with V = 8 that moves a score by 2^-20 of itself, no more than what exp and division leave uncertain.  By logits of 16
 // bits nothing moves at all: their FP32 form has 13 bits to spare, which hold the whole index.  A lane sorts its keys (two
 // instructions a comparison), and each round takes the largest of the 32 heads by one redux and moves that lane's list on.  Lists
-// hold four keys; a lane that has more and uses up four of them shows a last one that nothing exceeds, which counts as undecided.
+// hold four or five keys; a lane that has more and uses up its list shows a last one that nothing exceeds, which counts as undecided
+// (65536 tokens, 8 of 256 experts, of which 16 lanes hold what four of eight groups have: 0.4 % with lists of four).
 template <int V>
 struct Keys {
     static constexpr int PLACE_BITS = V <= 1 ? 0 : V <= 2 ? 1 : V <= 4 ? 2 : V <= 8 ? 3 : V <= 16 ? 4 : 5;
-    static constexpr int DEPTH = V < 4 ? V : 4;
+    static constexpr int DEPTH = V < 4 ? V : V == 8 ? 5 : 4;
     static constexpr uint32_t PLACES = (1u << PLACE_BITS) - 1, MORE = 0xffffffffu, NONE = 0x007fffffu;
 };
 
@@ -152,20 +158,24 @@ __device__ __forceinline__ void sort4(uint32_t (&k)[4]) {
     descending(k[1], k[3]);
     descending(k[1], k[2]);
 }
-// The largest of n keys (four at most), largest first.
-template <int N>
-__device__ __forceinline__ void largest(const uint32_t* k, uint32_t (&out)[N < 4 ? N : 4]) {
+// The D largest of N keys, largest first: N <= 4 all of them, of eight up to five, else four.
+template <int N, int D>
+__device__ __forceinline__ void largest(const uint32_t* k, uint32_t (&out)[D]) {
     if constexpr (N <= 4) {
+        static_assert(D == N, "all of them");
 #pragma unroll
         for (int i = 0; i < N; ++i) out[i] = k[i];
         if constexpr (N == 2) descending(out[0], out[1]);
         if constexpr (N == 4) sort4(out);
     } else {
-        uint32_t other[4];
-        largest<N / 2>(k, out);
-        largest<N / 2>(k + N / 2, other);
+        uint32_t one[4], other[4];
+        largest<N / 2, 4>(k, one);
+        largest<N / 2, 4>(k + N / 2, other);
+        // the larger of one's i-th and other's (3 - i)-th, the largest four of all eight, rise and fall; the fifth is the largest of the rest
+        if constexpr (D == 5)
+            out[4] = max(max(min(one[0], other[3]), min(one[1], other[2])), max(min(one[2], other[1]), min(one[3], other[0])));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) out[i] = max(out[i], other[3 - i]);     // the largest four, rising and falling
+        for (int i = 0; i < 4; ++i) out[i] = max(one[i], other[3 - i]);
         descending(out[0], out[2]);
         descending(out[1], out[3]);
         descending(out[0], out[1]);
@@ -184,10 +194,44 @@ __device__ __forceinline__ float reciprocal_fast(float x) {
     return y;
 }
 
+// The lane whose first key is the warp's largest, unless that stands for none, leaves it and `base` in place i of `found` and moves its
+// list on.  One predicate for all of it: a branch, or a select for every key, cost twice as much.
+template <int DEPTH>
+__device__ __forceinline__ void take_head(uint32_t (&head)[DEPTH], uint32_t rest, int& taken, uint32_t top, uint32_t none, uint32_t found,
+                                          int i, uint32_t base) {
+    const uint32_t to = found + 8 * i;
+    if constexpr (DEPTH == 1)
+        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.gt.u32 q, %3, %4;\n\tsetp.eq.and.u32 p, %0, %3, q;\n\t"
+                     "@p st.shared.v2.u32 [%5], {%3, %6};\n\t@p add.s32 %1, %1, 1;\n\t@p mov.u32 %0, %2;\n\t}"
+                     : "+r"(head[0]), "+r"(taken)
+                     : "r"(rest), "r"(top), "r"(none), "r"(to), "r"(base)
+                     : "memory");
+    else if constexpr (DEPTH == 2)
+        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.gt.u32 q, %4, %5;\n\tsetp.eq.and.u32 p, %0, %4, q;\n\t"
+                     "@p st.shared.v2.u32 [%6], {%4, %7};\n\t@p add.s32 %2, %2, 1;\n\t@p mov.u32 %0, %1;\n\t@p mov.u32 %1, %3;\n\t}"
+                     : "+r"(head[0]), "+r"(head[1]), "+r"(taken)
+                     : "r"(rest), "r"(top), "r"(none), "r"(to), "r"(base)
+                     : "memory");
+    else if constexpr (DEPTH == 4)
+        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.gt.u32 q, %6, %7;\n\tsetp.eq.and.u32 p, %0, %6, q;\n\t"
+                     "@p st.shared.v2.u32 [%8], {%6, %9};\n\t@p add.s32 %4, %4, 1;\n\t@p mov.u32 %0, %1;\n\t@p mov.u32 %1, %2;\n\t"
+                     "@p mov.u32 %2, %3;\n\t@p mov.u32 %3, %5;\n\t}"
+                     : "+r"(head[0]), "+r"(head[1]), "+r"(head[2]), "+r"(head[3]), "+r"(taken)
+                     : "r"(rest), "r"(top), "r"(none), "r"(to), "r"(base)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.gt.u32 q, %7, %8;\n\tsetp.eq.and.u32 p, %0, %7, q;\n\t"
+                     "@p st.shared.v2.u32 [%9], {%7, %10};\n\t@p add.s32 %5, %5, 1;\n\t@p mov.u32 %0, %1;\n\t@p mov.u32 %1, %2;\n\t"
+                     "@p mov.u32 %2, %3;\n\t@p mov.u32 %3, %4;\n\t@p mov.u32 %4, %6;\n\t}"
+                     : "+r"(head[0]), "+r"(head[1]), "+r"(head[2]), "+r"(head[3]), "+r"(head[4]), "+r"(taken)
+                     : "r"(rest), "r"(top), "r"(none), "r"(to), "r"(base)
+                     : "memory");
+}
+
 // What experts are chosen by: the logits themselves, or (with a bias, or groups that count with two experts) scores of them.
 enum ChosenBy { LOGITS, SOFTMAX, SIGMOID };
 
-// l[j]: the lane's logits, -inf where there is none to choose; bias[j]: their biases; base: the lane's first expert; found: the
+// l[j]: the lane's logits, -inf where there is none to choose (SIGMOID: any that cannot be chosen); bias[j]: their biases; base: the lane's first expert; found: the
 // warp's place for the rounds' keys and lanes.
 template <typename T, int V, ChosenBy BY>
 __device__ __forceinline__ bool select_in_32_bits(const SelectArgs& a, const float (&l)[V], const float (&bias)[V], int lane, int base,
@@ -223,7 +267,7 @@ __device__ __forceinline__ bool select_in_32_bits(const SelectArgs& a, const flo
                 s = reciprocal_fast(1.f + exp2_fast(l[j] * -LOG2E));
             else
                 s = (l[j] == top ? 1.f : exp2_fast((l[j] - top) * LOG2E)) * part;
-            const float c = l[j] > -INFINITY ? s + bias[j] : -INFINITY;
+            const float c = l[j] > (BY == SIGMOID ? Lowest<T>::value() : -INFINITY) ? s + bias[j] : -INFINITY;
             key[j] = (key_of(c) & ~LOW) | (low0 - j);
         }
     } else {
@@ -231,7 +275,7 @@ __device__ __forceinline__ bool select_in_32_bits(const SelectArgs& a, const flo
         for (int j = 0; j < V; ++j) key[j] = (key_of(l[j]) & ~LOW) | (low0 - j);
     }
     uint32_t head[K::DEPTH];
-    largest<V>(key, head);
+    largest<V, K::DEPTH>(key, head);
     uint32_t rest = V > K::DEPTH && head[K::DEPTH - 1] > K::NONE ? K::MORE : 0u;
     constexpr float SPREAD = SCORES ? (float)(1u << K::PLACE_BITS) * 0x1p-21f : 0.f;
     bool sure = true;
@@ -257,7 +301,7 @@ __device__ __forceinline__ bool select_in_32_bits(const SelectArgs& a, const flo
         const uint32_t next = __reduce_max_sync(0xffffffffu, left);
         if (next) {
             if constexpr (SCORES) {
-                size = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(size)));
+                size = __uint_as_float(__reduce_max_sync(0xffffffffu, group >= next ? __float_as_uint(size) : 0u));
                 sure = value_of(last & ~31u) - value_of(next & ~31u) > 2.f * uncertain + size * (SPREAD + 0x1p-16f);
             } else {
                 sure = WHOLE || (last >> 5) != (next >> 5);
@@ -269,24 +313,24 @@ __device__ __forceinline__ bool select_in_32_bits(const SelectArgs& a, const flo
             rest = 0u;
         }
     }
-    // Rounds.  Lanes whose heads are equal move on together: the keys that are lost so are counted, and leave it undecided.
-    int taken = 0, rounds = 0;
-    for (; rounds <= a.k; ++rounds) {
-        const uint32_t top = __reduce_max_sync(0xffffffffu, head[0]);
-        if (top <= K::NONE) break;
-        if (head[0] == top) {
-            found[rounds] = make_uint2(top, (uint32_t)base);
+    // Rounds, one past the last expert (and up to two more).  Lanes whose heads are equal move on together: the keys that are lost so
+    // are counted, and leave it undecided.
+    const uint32_t at = (uint32_t)__cvta_generic_to_shared(found);
+    if (lane < MAX_ROUNDS) found[lane] = make_uint2(0u, 0u);
+    __syncwarp();
+    int taken = 0;
 #pragma unroll
-            for (int d = 0; d + 1 < K::DEPTH; ++d) head[d] = head[d + 1];
-            head[K::DEPTH - 1] = rest;
-            ++taken;
-        }
+    for (int i = 0; i < MAX_ROUNDS; ++i) {
+        if (i % 3 == 0 && i > a.k) break;
+        const uint32_t top = __reduce_max_sync(0xffffffffu, head[0]);
+        take_head<K::DEPTH>(head, rest, taken, top, K::NONE, at, i, (uint32_t)base);
     }
     __syncwarp();
-    const uint2 choice = lane < rounds ? found[lane] : make_uint2(0u, 0u);
+    const uint2 choice = lane < MAX_ROUNDS ? found[lane] : make_uint2(0u, 0u);
     const uint32_t best = choice.x, after = __shfl_down_sync(0xffffffffu, best, 1);
+    const int rounds = __popc(__ballot_sync(0xffffffffu, best != 0u));
     __syncwarp();
-    sure = sure && best != K::MORE;
+    sure = sure && (lane > a.k || best != K::MORE);
     if (!WHOLE && lane < a.k && after) {
         if constexpr (SCORES) {
             const float high = value_of(best & ~LOW);
@@ -301,10 +345,11 @@ __device__ __forceinline__ bool select_in_32_bits(const SelectArgs& a, const flo
 }
 
 // Weights of chosen experts, and the answer.  `width` lanes, a power of two, have the experts of one token (-1: none), rank r in
-// the r-th of them.  Renormalised weights are computed from the chosen logits alone, relative to the largest, so they do not vanish
+// the r-th of them; whole: the row's largest logit and sum of exponentials, for softmax weights that are not renormalised.
+// Renormalised weights are computed from the chosen logits alone, relative to the largest, so they do not vanish
 // where all scores do.
 template <typename T>
-__device__ __forceinline__ void store_choice(const SelectArgs& a, long long t, int r, int mine, int width, bool live) {
+__device__ __forceinline__ void store_choice(const SelectArgs& a, long long t, int r, int mine, int width, bool live, float2 whole) {
     const T* row = static_cast<const T*>(a.logits) + t * a.ld;
     const float l = live && mine >= 0 ? to_float(row[mine]) : -INFINITY;
     float w = 0.f;
@@ -322,21 +367,8 @@ __device__ __forceinline__ void store_choice(const SelectArgs& a, long long t, i
         w = mine >= 0 ? w / sum : 0.f;
     } else if (a.sigmoid) {
         w = mine >= 0 ? 1.f / (1.f + expf(-l)) : 0.f;
-    } else if (live) {
-        // the sum over all experts of the row, by the token's own lanes
-        float all = -INFINITY, sum = 0.f;
-        for (int e = r; e < a.E; e += width) {
-            const float v = to_float(row[e]);
-            all = v > Lowest<T>::value() ? fmaxf(all, v) : all;
-        }
-        const unsigned lanes = width == 32 ? 0xffffffffu : ((1u << width) - 1u) << ((threadIdx.x & 31) & ~(width - 1));
-        for (int off = width >> 1; off >= 1; off >>= 1) all = fmaxf(all, __shfl_xor_sync(lanes, all, off));
-        for (int e = r; e < a.E; e += width) {
-            const float v = to_float(row[e]);
-            if (v > Lowest<T>::value()) sum += v == all ? 1.f : expf(v - all);
-        }
-        for (int off = width >> 1; off >= 1; off >>= 1) sum += __shfl_xor_sync(lanes, sum, off);
-        w = mine >= 0 ? (l == all ? 1.f : expf(l - all)) / sum : 0.f;
+    } else {
+        w = mine >= 0 ? (l == whole.x ? 1.f : expf(l - whole.x)) / whole.y : 0.f;
     }
     if (live && r < a.k) {
         a.gate[t * a.k + r] = mine;
@@ -345,8 +377,8 @@ __device__ __forceinline__ void store_choice(const SelectArgs& a, long long t, i
     }
 }
 
-// The lane's V logits of a row; -inf for an expert that cannot be chosen, or is not there.
-template <typename T, int V>
+// The lane's V logits of a row; -inf for an expert that is not there, or (MASK) cannot be chosen.
+template <typename T, int V, bool MASK>
 __device__ __forceinline__ void load_logits(const SelectArgs& a, long long t, int first, int count, float (&l)[V]) {
     const T* row = static_cast<const T*>(a.logits) + t * a.ld + first;
     constexpr int N = V * sizeof(T) >= 16 ? 16 / (int)sizeof(T) : V;
@@ -362,17 +394,20 @@ __device__ __forceinline__ void load_logits(const SelectArgs& a, long long t, in
 #pragma unroll
         for (int j = 0; j < V; ++j) l[j] = j < count ? to_float(row[j]) : -INFINITY;
     }
+    if constexpr (MASK)
 #pragma unroll
-    for (int j = 0; j < V; ++j) l[j] = l[j] > Lowest<T>::value() ? l[j] : -INFINITY;    // NaN too
+        for (int j = 0; j < V; ++j) l[j] = l[j] > Lowest<T>::value() ? l[j] : -INFINITY;    // NaN too
 }
 
 // A warp per token, tokens a grid apart, 32 to a warp before the block meets.  As many tokens as fit into the lanes (four with 5 to
 // 8 experts each) then get their weights together: by token that took 10 of 45 us (65536 tokens, 8 of 256 experts).  Tokens
-// that 32 bits leave undecided wait until the block's are done; in the loop itself that choice cost every token its registers, 20 us.
+// that 32 bits leave undecided wait until the block's are done, and its warps share them; in the loop itself that choice cost every
+// token its registers, 20 us, and by each warp after a few tokens 4 us more than so.
 template <typename T, int V, ChosenBy BY>
 __global__ void __launch_bounds__(SELECT_WARPS * 32, V <= 8 ? 4 : V <= 16 ? 3 : 2) select_topk_kernel(const __grid_constant__ SelectArgs a) {
-    __shared__ uint2 s_found[SELECT_WARPS][17];
+    __shared__ uint2 s_found[SELECT_WARPS][MAX_ROUNDS];
     __shared__ int s_choice[SELECT_WARPS][32];
+    __shared__ float2 s_row[SELECT_WARPS][32];                      // softmax of all experts, by turn: the largest logit, and the sum
     __shared__ int s_open[SELECT_WARPS * 32], s_open_count;         // undecided tokens: warp and turn
     pdl_trigger();
     pdl_wait();
@@ -387,36 +422,46 @@ __global__ void __launch_bounds__(SELECT_WARPS * 32, V <= 8 ? 4 : V <= 16 ? 3 : 
     }
     const long long step = (long long)gridDim.x * SELECT_WARPS;
     const int width = 1 << a.width_log2, batch = 32 >> a.width_log2, r = lane & (width - 1);
+    const bool whole_sum = !a.sigmoid && !a.renormalise;
     for (long long t0 = (long long)blockIdx.x * SELECT_WARPS; t0 < a.T; t0 += 32 * step) {      // the block's next 32 turns
         if (threadIdx.x == 0) s_open_count = 0;
         __syncthreads();
         for (int turn = 0; turn < 32 && t0 + warp + turn * step < a.T; turn += batch) {
             s_choice[warp][lane] = -2;
             __syncwarp();
-            for (int i = 0; i < batch; ++i) {
-                const long long t = t0 + warp + (turn + i) * step;
-                if (t >= a.T) break;
+            long long t = t0 + warp + turn * step;
+            for (int i = 0; i < batch && t < a.T; ++i, t += step) {
                 float l[V];
-                load_logits<T, V>(a, t, first, count, l);
+                load_logits<T, V, BY != SIGMOID>(a, t, first, count, l);
+                if (BY != SIGMOID && whole_sum) {
+                    float top = l[0], sum = 0.f;
+#pragma unroll
+                    for (int j = 1; j < V; ++j) top = fmaxf(top, l[j]);
+                    top = warp_max(top);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) sum += l[j] == top ? 1.f : expf(l[j] - top);
+                    sum = warp_xor_sum(sum);
+                    if (lane == 0) s_row[warp][turn + i] = make_float2(top, sum);
+                }
                 int mine = -1;
-                if (a.k <= 16 && select_in_32_bits<T, V, BY>(a, l, bias, lane, first, s_found[warp], mine)) {
+                if (a.k <= MAX_FAST_K && select_in_32_bits<T, V, BY>(a, l, bias, lane, first, s_found[warp], mine)) {
                     if (lane < width) s_choice[warp][i * width + lane] = mine;
                 } else if (lane == 0) {
                     s_open[atomicAdd(&s_open_count, 1)] = warp * 32 + turn + i;
                 }
             }
             __syncwarp();
-            const int mine = s_choice[warp][lane];
-            const long long t = t0 + warp + (turn + (lane >> a.width_log2)) * step;
-            store_choice<T>(a, min(t, a.T - 1), r, mine, width, mine != -2);
+            const int mine = s_choice[warp][lane], i = turn + (lane >> a.width_log2);
+            store_choice<T>(a, min(t0 + warp + i * step, a.T - 1), r, mine, width, mine != -2, s_row[warp][i]);
             __syncwarp();
         }
         __syncthreads();
         const int open = s_open_count;
         for (int i = warp; i < open; i += SELECT_WARPS) {
-            const long long t = t0 + (s_open[i] >> 5) + (s_open[i] & 31) * step;
+            const int of = s_open[i] >> 5, turn = s_open[i] & 31;
+            const long long t = t0 + of + turn * step;
             const int mine = select_in_64_bits<T, V>(a, t, lane);
-            store_choice<T>(a, t, lane, mine, 32, true);
+            store_choice<T>(a, t, lane, mine, 32, true, s_row[of][turn]);
         }
         __syncthreads();
     }
