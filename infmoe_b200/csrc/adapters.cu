@@ -640,14 +640,14 @@ struct TcShape {
     static constexpr int STAGE1 = (TC_ROWS + RP) * 128;
     static constexpr int S1 = RP == 128 ? 3 : 4;
     static constexpr int SMEM1 = S1 * STAGE1 + 1024;                // + slack for 1024-byte alignment
-    static constexpr int ATOMS = (RP + 63) / 64;                    // 128-byte parts of a row of A x, and of B
-    static constexpr int V_BYTES = ATOMS * TC_ROWS * 128;           // twice: first and second parts
+    static constexpr int ATOMS = (RP + 63) / 64;                    // 128-byte parts of a row of B
     static constexpr int Y_BYTES = TC_ROWS * 128;
     static constexpr int STAGE2 = Y_BYTES + ATOMS * COLUMNS * 128;
     static constexpr int S2 = 3;
-    static constexpr int SMEM2 = 2 * V_BYTES + S2 * STAGE2 + 1024;
-    static constexpr int PER_SM1 = 2, PER_SM2 = RP == 128 ? 1 : 2;  // blocks an SM has room for
-    static constexpr uint32_t TMEM1 = RP < 32 ? 32 : RP, TMEM2 = COLUMNS;   // columns of tensor memory
+    static constexpr int SMEM2 = S2 * STAGE2 + 1024;
+    static constexpr int PER_SM1 = 2, PER_SM2 = RP == 128 ? 2 : 3;  // blocks an SM has room for
+    // Columns of tensor memory: sums, and in the second kernel A x, two values to a column, first parts and second parts.
+    static constexpr uint32_t TMEM1 = RP < 32 ? 32 : RP, TMEM2 = COLUMNS + RP <= 128 ? 128 : 256;
 };
 
 template <typename T>
@@ -660,6 +660,21 @@ __device__ __forceinline__ void tmem_alloc(uint32_t* where, uint32_t columns) {
 __device__ __forceinline__ void tmem_free(uint32_t base, uint32_t columns) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns) : "memory");
 }
+
+// D[tmem] (+)= A[tmem] * B[smem]^T: 16-bit operands, a row of A to a lane, two values of K to a column; B K-major; K = 16.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// A lane's four columns of tensor memory.
+__device__ __forceinline__ void tmem_st4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // A x of a tile.  Tensor memory is allocated before the next kernel may start: blocks that hold some of it never wait for one that
 // still needs some.
@@ -774,9 +789,10 @@ __global__ void __launch_bounds__(APPLY_THREADS) adapter_down_tc_kernel(const Ap
     if (warp == 0) tmem_free(tmem, S::TMEM1);
 }
 
-// y + scale B v of a tile's share of the columns.  Starts under adapter_down_tc_kernel, like adapter_up_kernel.
+// y + scale B v of a tile's share of the columns.  Starts under adapter_down_tc_kernel, like adapter_up_kernel.  A x is an operand
+// from tensor memory: the shared memory that it took, 32 KB, holds a third block's stages.
 template <typename T, int RP, bool FAST>
-__global__ void __launch_bounds__(APPLY_THREADS) adapter_up_tc_kernel(const ApplyArgs p) {
+__global__ void __launch_bounds__(APPLY_THREADS, TcShape<RP>::PER_SM2) adapter_up_tc_kernel(const ApplyArgs p) {
     using S = TcShape<RP>;
     extern __shared__ __align__(128) char smem_raw[];
     __shared__ __align__(8) uint64_t s_done;
@@ -784,8 +800,8 @@ __global__ void __launch_bounds__(APPLY_THREADS) adapter_up_tc_kernel(const Appl
     __shared__ int s_abort, s_pos[TC_ROWS];
     __shared__ float s_unscale[TC_ROWS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, v_at = base, ring = base + 2 * S::V_BYTES;
-    char* const base_ptr = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    char* const ring_ptr = smem_raw + (ring - smem_u32(smem_raw));
     const int tile_index = blockIdx.x / p.col_split, share = blockIdx.x % p.col_split;
     const int4 tile = p.tiles[tile_index];
     const int token = tid < TC_ROWS ? p.rows[tile_index * TC_ROWS + tid] : 0;
@@ -854,30 +870,37 @@ __global__ void __launch_bounds__(APPLY_THREADS) adapter_up_tc_kernel(const Appl
     pdl_wait();
     pdl_trigger();
 
-    // A x: the shares of all blocks, as first and second parts.  A thread has four columns of a row, and of rows ROWS further on.
+    // A x: the shares of all blocks, as first and second parts, through the ring's last slot, which the loop's first turn fills.  The
+    // sums by neighbours (a thread has four columns of a row, and of rows ROWS further on), then to tensor memory by rows: a thread
+    // half of a row, the one whose lane is its warp's to write.
+    const int row = (warp & 3) * 32 + lane, half = warp >> 2;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     {
-        constexpr int LANES = RP / 4, ROWS = APPLY_THREADS / LANES, PASSES = TC_ROWS / ROWS, GROUP = PASSES < 8 ? PASSES : 8;
+        constexpr int PART_ROWS = RP == 128 ? 32 : 64, PITCH = RP * 2 + 16;     // rows at a time, and bytes of a row
+        static_assert(2 * PART_ROWS * PITCH <= S::STAGE2, "both parts fit into a slot");
+        constexpr int LANES = RP / 4, ROWS = APPLY_THREADS / LANES, PASSES = PART_ROWS / ROWS, TOGETHER = PASSES <= 1 ? 4 : 2;
+        char* const staged = ring_ptr + (S::S2 - 1) * S::STAGE2;
         const int col = tid % LANES * 4, r0 = tid / LANES;
-        const float* const from = p.sums + ((size_t)tile_index * TC_ROWS + r0) * RP + col;
         const size_t stride = (size_t)p.tile_count * (TC_ROWS * RP);
 #pragma unroll 1
-        for (int g0 = 0; g0 < PASSES; g0 += GROUP) {
-            float4 v[GROUP];
+        for (int part = 0; part < TC_ROWS; part += PART_ROWS) {
+            if (part >= tile.z) break;
+            const float* const from = p.sums + ((size_t)tile_index * TC_ROWS + part + r0) * RP + col;
+            float4 v[PASSES];
 #pragma unroll
-            for (int i = 0; i < GROUP; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            constexpr int TOGETHER = GROUP <= 2 ? 8 : GROUP <= 4 ? 4 : 2;
+            for (int i = 0; i < PASSES; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll TOGETHER
             for (int q = 0; q < p.k_split; ++q) {
 #pragma unroll
-                for (int i = 0; i < GROUP; ++i) {
-                    if (r0 + (g0 + i) * ROWS >= tile.z) continue;
-                    const float4 o = __ldcg(reinterpret_cast<const float4*>(from + q * stride + (g0 + i) * ROWS * RP));
+                for (int i = 0; i < PASSES; ++i) {
+                    if (part + r0 + i * ROWS >= tile.z) continue;
+                    const float4 o = __ldcg(reinterpret_cast<const float4*>(from + q * stride + i * ROWS * RP));
                     v[i] = make_float4(v[i].x + o.x, v[i].y + o.y, v[i].z + o.z, v[i].w + o.w);
                 }
             }
 #pragma unroll
-            for (int i = 0; i < GROUP; ++i) {
-                const int r = r0 + (g0 + i) * ROWS;
+            for (int i = 0; i < PASSES; ++i) {
+                const int r = r0 + i * ROWS;
                 if (col >= rank) v[i].x = 0.f;
                 if (col + 1 >= rank) v[i].y = 0.f;
                 if (col + 2 >= rank) v[i].z = 0.f;
@@ -888,23 +911,34 @@ __global__ void __launch_bounds__(APPLY_THREADS) adapter_up_tc_kernel(const Appl
                     for (int off = LANES / 2; off >= 1; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
                     const int e = row_exponent(most);
                     const float up = exp2_int(e);
-                    if (col == 0 && r < tile.z) s_unscale[r] = exp2_int(-e);
+                    if (col == 0) s_unscale[part + r] = exp2_int(-e);
                     v[i] = make_float4(v[i].x * up, v[i].y * up, v[i].z * up, v[i].w * up);
                 }
-                if (r >= tile.z) continue;
-                char* const to = base_ptr + (col / 64) * (TC_ROWS * 128) + r * 128 + (((col % 64 / 8) ^ (r & 7)) << 4) + col % 8 * 2;
+                char* const to = staged + r * PITCH + col * 2;
                 *reinterpret_cast<uint2*>(to) = make_uint2(pack_pair<T>(v[i].x, v[i].y), pack_pair<T>(v[i].z, v[i].w));
-                *reinterpret_cast<uint2*>(to + S::V_BYTES) = make_uint2(pack_pair<T>(rest_of<T>(v[i].x), rest_of<T>(v[i].y)),
-                                                                        pack_pair<T>(rest_of<T>(v[i].z), rest_of<T>(v[i].w)));
+                *reinterpret_cast<uint2*>(to + PART_ROWS * PITCH) = make_uint2(pack_pair<T>(rest_of<T>(v[i].x), rest_of<T>(v[i].y)),
+                                                                               pack_pair<T>(rest_of<T>(v[i].z), rest_of<T>(v[i].w)));
             }
+            __syncthreads();
+            if ((warp & 3) * 32 / PART_ROWS == part / PART_ROWS) {
+#pragma unroll
+                for (int c = 0; c < RP; c += 16) {                  // 16 bytes, eight columns of this half
+                    const char* at = staged + (row - part) * PITCH + half * RP + c;
+                    const uint4 hi = *reinterpret_cast<const uint4*>(at), lo = *reinterpret_cast<const uint4*>(at + PART_ROWS * PITCH);
+                    const uint32_t to = lanes + S::COLUMNS + half * (RP / 4) + c / 4;
+                    tmem_st4(to, hi.x, hi.y, hi.z, hi.w);
+                    tmem_st4(to + RP / 2, lo.x, lo.y, lo.z, lo.w);
+                }
+                tmem_st_wait();
+            }
+            __syncthreads();
         }
     }
-    // the loop's first fence and barrier hand A x to the MMAs
+    const float factor = std::is_same_v<T, __half> && row < tile.z ? scale * s_unscale[row] : scale;
+    // the loop's first fences and barrier hand A x to the MMAs
 
     const uint32_t idesc = make_idesc(TC_ROWS, S::COLUMNS, operand_format<T>());
-    const int row = (warp & 3) * 32 + lane, half = warp >> 2;       // of the last step: a row's 32 columns
-    float factor = scale;
-    bool ok = true, first = true;
+    bool ok = true;
     int slot = 0, before = S::S2 - 1;
     T* const out_base = static_cast<T*>(p.out);
     for (int c = 0; c < col_stages; ++c) {
@@ -919,24 +953,21 @@ __global__ void __launch_bounds__(APPLY_THREADS) adapter_up_tc_kernel(const Appl
             for (int part = 1; part >= 0; --part)                   // the second parts first
 #pragma unroll
                 for (int j = 0; j < RP / 16; ++j) {
-                    const uint64_t dv = make_smem_desc(v_at + part * S::V_BYTES + j / 4 * (TC_ROWS * 128)) + 2 * (j & 3);
                     const uint64_t db = make_smem_desc(stage + S::Y_BYTES + j / 4 * (S::COLUMNS * 128)) + 2 * (j & 3);
-                    umma_f16_ss(tmem, dv, db, idesc, part == 0 || j > 0);
+                    umma_f16_ts(tmem, tmem + S::COLUMNS + part * (RP / 2) + 8 * j, db, idesc, part == 0 || j > 0);
                 }
             umma_commit(smem_u32(&s_done));
         }
         if (ok) fetch(c + S::S2 - 1, before);
         else copies_commit();
-        if (std::is_same_v<T, __half> && first && row < tile.z) factor = scale * s_unscale[row];
-        first = false;
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_done), c & 1, &s_abort));
         tc_fence_after();
-        char* const tile_y = base_ptr + (stage - base);
+        char* const tile_y = ring_ptr + (stage - ring);
         if (ok) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 uint32_t sum[16];
-                tmem_ld16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 32 + h * 16, sum);
+                tmem_ld16(lanes + half * 32 + h * 16, sum);
                 tmem_ld_wait();
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
@@ -1013,7 +1044,7 @@ int launch_few(ApplyArgs a, cudaStream_t stream) {
 template <typename T, int RP, bool FAST>
 int launch_many(ApplyArgs a, cudaStream_t stream) {
     using S = TcShape<RP>;
-    a.k_split = split(a.tile_count, S::PER_SM1, (a.d_in + S::K_CHUNK - 1) / S::K_CHUNK, MAX_K_SPLIT);
+    a.k_split = split(a.tile_count, S::PER_SM1, (a.d_in + S::K_CHUNK - 1) / S::K_CHUNK, 4);   // every block of the second kernel adds the shares up
     a.col_split = split(a.tile_count, S::PER_SM2, (a.d_out + S::COLUMNS - 1) / S::COLUMNS, 1 << 20);
     return launch_pair(adapter_down_tc_kernel<T, RP, FAST>, adapter_up_tc_kernel<T, RP, FAST>, a, S::SMEM1, S::SMEM2, stream);
 }

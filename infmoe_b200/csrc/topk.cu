@@ -609,8 +609,9 @@ int launch_scatter_topk_rows(long long rows, int k, long long row_bytes, const v
 template <typename Vec>
 int launch_scatter_topk_vec(long long rows, int k, long long row_bytes, const void* x, long long ldx_bytes, const int* pos,
                             const int* valid_rows, void* routed, int* row_of, cudaStream_t stream) {
-    // Four vectors to a thread where there is enough to do for all of them (32768 rows of 8 KB: one 82 us, two 61, four 57, eight 66);
-    // one where blocks are few (512 rows: 4.7 us either way, 64: 2.4).
+    // Four vectors to a thread where there is enough to do for all of them (32768 rows of 8 KB: one 82 us, two 61, four 57, eight 66;
+    // four of one row instead of four rows: 16384 rows of 16 KB 69 instead of 60); one where blocks are few (512 rows of 8 KB: 4.7 us
+    // either way, 64: 2.4).
     if (rows * row_bytes > (8 << 20))
         return launch_scatter_topk_rows<Vec, 4>(rows, k, row_bytes, x, ldx_bytes, pos, valid_rows, routed, row_of, stream);
     return launch_scatter_topk_rows<Vec, 1>(rows, k, row_bytes, x, ldx_bytes, pos, valid_rows, routed, row_of, stream);
