@@ -55,6 +55,12 @@ int dtype_code(const at::Tensor& t) {
     }
 }
 
+// A size that the C ABI takes in 32 bits.
+int32_t size32(int64_t n, const char* what) {
+    if (n > INT32_MAX) refuse("%s is too large (%lld)", what, (long long)n);
+    return (int32_t)n;
+}
+
 // Rows of a CUDA tensor [..., width] and the stride between them: any stride for [T, width], contiguous otherwise.
 struct Rows {
     int64_t count, ld;
@@ -182,7 +188,7 @@ PyObject* scatter_topk(PyObject* const* a) {
     const at::Tensor out = output(a[4], {rows.count * k, D}, x.scalar_type(), device, "out");
     const at::Tensor row_of = output(a[5], {rows.count, k}, at::kInt, device, "row_of");
     const On on(x);
-    check(infmoe_expert_scatter_topk(rows.count, (int32_t)k, (int32_t)D, dtype_code(x), x.data_ptr(), rows.ld, (const int32_t*)pos.data_ptr(),
+    check(infmoe_expert_scatter_topk(rows.count, (int32_t)k, size32(D, "D"), dtype_code(x), x.data_ptr(), rows.ld, (const int32_t*)pos.data_ptr(),
                                      (const int32_t*)offset.data_ptr() + (offset.numel() - 1), out.data_ptr(), (int32_t*)row_of.data_ptr(),
                                      on.stream));
     return pair(out, row_of);
@@ -204,7 +210,7 @@ PyObject* combine_topk(PyObject* const* a) {
     const int dtype = dtype_code(rows);
     const at::Tensor out = output(a[5], shape, rows.scalar_type(), device, "out");
     const On on(rows);
-    check(infmoe_expert_combine_topk(weight.numel() / k, (int32_t)k, (int32_t)D, dtype, rows.data_ptr(), rows.size(0),
+    check(infmoe_expert_combine_topk(weight.numel() / k, size32(k, "top_k"), size32(D, "D"), dtype, rows.data_ptr(), rows.size(0),
                                      (const float*)weight.data_ptr(), (const int32_t*)data(gate), (const int32_t*)data(row_of),
                                      data(residual), out.data_ptr(), on.stream));
     return wrap(out);

@@ -500,6 +500,7 @@ int launch_select_type(const SelectArgs& a, int per_lane, cudaStream_t stream) {
 // ---- rows to k experts and back ------------------------------------------------------------------
 
 constexpr int ROW_THREADS = 256;
+constexpr int MAX_TOKEN_LEN = 65535 * ROW_THREADS;   // parts of a row that a grid's second dimension can count, one element to a thread
 
 // How a block of ROW_THREADS shares out rows of `vecs` vectors: rows_per_block whole rows, or (one row per block) parts of a
 // row along grid.y.
@@ -728,8 +729,9 @@ int infmoe_expert_scatter_topk(int64_t T, int32_t top_k, int32_t token_len, int3
                   token_len, (long long)ld, dtype);
         return INFMOE_ERR_INVALID_ARGUMENT;
     }
-    if (T > 0x7fffffffLL / top_k) {
-        set_error("expert_scatter_topk: %lld tokens of %d slots are too many for 32-bit slot indices", (long long)T, top_k);
+    if (T > 0x7fffffffLL / top_k || token_len > MAX_TOKEN_LEN) {
+        set_error("expert_scatter_topk: %lld tokens of %d slots are too many for 32-bit slot indices, or rows of %d elements too long",
+                  (long long)T, top_k, token_len);
         return INFMOE_ERR_UNSUPPORTED;
     }
     if (T == 0) return INFMOE_OK;
@@ -746,8 +748,9 @@ int infmoe_expert_combine_topk(int64_t T, int32_t top_k, int32_t token_len, int3
                   (long long)rows, top_k, token_len, dtype);
         return INFMOE_ERR_INVALID_ARGUMENT;
     }
-    if (T > 0x7fffffffLL / top_k) {
-        set_error("expert_combine_topk: %lld tokens of %d slots are too many for 32-bit slot indices", (long long)T, top_k);
+    if (T > 0x7fffffffLL / top_k || token_len > MAX_TOKEN_LEN) {
+        set_error("expert_combine_topk: %lld tokens of %d slots are too many for 32-bit slot indices, or rows of %d elements too long",
+                  (long long)T, top_k, token_len);
         return INFMOE_ERR_UNSUPPORTED;
     }
     if (T == 0) return INFMOE_OK;

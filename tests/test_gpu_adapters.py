@@ -356,3 +356,25 @@ def test_many_tokens_captured_behind_a_layer():
         assert torch.equal(out, step())
     del g
     layer.terminate()
+
+
+def test_rows_past_32_bits():
+    """Elements of x, y and out beyond 2^32 of their tensors."""
+    T, ld, d, r = (1 << 20) + 50, 4104, 64, 16
+    t = torch.bfloat16
+    rng = np.random.default_rng(31)
+    x = torch.zeros(T, ld, dtype=t, device="cuda")                  # 8.6 GB
+    x[-70:, :d] = whole(rng, (70, d), 2, t)
+    y = torch.zeros(T, d, dtype=t, device="cuda")
+    y[-70:] = whole(rng, (70, d), 50, t)
+    a, b = whole(rng, (2, r, d), 2, t), whole(rng, (2, d, r), 1, t)
+    at = np.full(T, -1, np.int32)
+    at[-70:] = owners(rng, 70, 2, 7)
+    adapters = Adapters(a, b)
+    plan = adapters.plan(torch.from_numpy(at).cuda())
+    got = adapters.apply(x[:, :d], y, plan)
+    check_exact(got[-70:], reference(x[-70:, :d], y[-70:], a, b, 1, None, at[-70:]), t)
+    assert not got[:-70].any()
+    into = x[:, 2000:2000 + d]                                      # rows apart on the way out too
+    adapters.apply(x[:, :d], y, plan, out=into)
+    assert torch.equal(into, got)

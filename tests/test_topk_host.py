@@ -1,5 +1,7 @@
 """What the operators for several experts per token and for adapters refuse, before any device work."""
 import ctypes
+import os
+import re
 
 import numpy as np
 import pytest
@@ -143,3 +145,40 @@ def test_reference_choices_by_hand():
     assert gate.tolist() == [[0]] and abs(w[0, 0] - 1 / (1 + np.exp(-1))) < 1e-15
     gate, _ = topk_ref.select(np.array([[5.0, -9, 2, 2.5]]), -1e38, 1, "sigmoid", None, 2, 1, 2)
     assert gate.tolist() == [[3]]                                # 0.993 + 0.0001 against 0.881 + 0.924
+
+
+def test_rows_longer_than_a_grid_can_count_are_refused():
+    lib = capi.lib()
+    assert lib.infmoe_expert_scatter_topk(3, 2, 1 << 25, 0, SOME, 1 << 25, SOME, SOME, SOME, SOME, None) == 6
+    assert lib.infmoe_expert_combine_topk(3, 2, 1 << 25, 0, SOME, 6, SOME, None, None, None, 2 * SOME, None) == 6
+    assert _apply(d_in=(1 << 24) + 1, ldx=1 << 25) == 6
+    assert _apply(d_out=(1 << 24) + 1, ldy=1 << 25, ldo=1 << 25) == 6
+
+
+def _body(source, kernel):
+    text = re.sub(r"//[^\n]*", "", source)
+    at = text.index("{", text.index(f"{kernel}(const ApplyArgs p)"))
+    depth, i = 0, at
+    while True:
+        depth += {"{": 1, "}": -1}.get(text[i], 0)
+        i += 1
+        if depth == 0:
+            return text[at:i]
+
+
+def test_adapters_second_kernel_may_start_early():
+    """It reads, before its own wait, what was there before the first one's, which therefore triggers behind its wait; and the first
+    one, where it takes tensor memory, has it before it triggers: blocks that hold some must not keep others from theirs."""
+    with open(os.path.join(os.path.dirname(capi.LIB_PATH), "csrc", "adapters.cu")) as f:
+        source = f.read()
+    for kernel in ("adapter_down_kernel", "adapter_down_tc_kernel"):
+        body = _body(source, kernel)
+        assert body.index("pdl_wait()") < body.index("pdl_trigger()"), kernel
+    for kernel in ("adapter_down_tc_kernel", "adapter_up_tc_kernel"):
+        body = _body(source, kernel)
+        assert body.index("tmem_alloc(") < body.rindex("pdl_trigger()"), kernel
+    for kernel in ("adapter_up_kernel", "adapter_up_tc_kernel"):        # shares of A x, and every store to memory
+        body = _body(source, kernel)
+        first_wait = body.index("pdl_wait()")
+        assert body.index("p.sums") > first_wait and body.index("out_base + (long long)") > first_wait, kernel
+        assert "mbar_wait" not in body[:first_wait]
