@@ -1,6 +1,13 @@
 // Low-rank adapters of many requests at once, beside a shared projection: out[t] = y[t] + scale[a] B[a] (A[a] x[t]) with
 // a the adapter of token t.  Tokens are grouped by adapter with the layer's own dispatch (an adapter takes the place of an
 // expert); the plan that comes of it holds for every projection of the batch.
+//
+// Two kernels: v = A x, d_in shared out over blocks whose sums go through a workspace and are added in a fixed order, then
+// y + scale B v, which starts under the first and fetches y and B meanwhile.  A token costs 2 r (d_in + d_out) products for its
+// (d_in + 2 d_out) elements, so memory bounds large batches and the latency of two kernels small ones.  Device time and what
+// the bytes take at the copy rate, us: 64 tokens and as many adapters of rank 16, 4096 x 4096, BF16 7.5 and 1.9; 4096 tokens, 8 of
+// rank 16 21.8 and 15.3; 777 tokens of up to rank 24, 1000 x 2724, FP32 14.3 and 3.2; 16384 tokens of rank 64, 4096 x 10240, FP16
+// 182 and 129.  As one kernel, with clusters and distributed shared memory, the second of these took 25.3.
 #include <cfloat>
 #include <climits>
 #include <type_traits>
@@ -210,16 +217,17 @@ struct ApplyShape {
 
     static constexpr int SUBS = 2, K_CHUNK = SUBS * 128 / SIZE;     // 128-byte parts of K in a stage
     static constexpr int STAGE1 = SUBS * (M + RP) * 128;
-    static constexpr int S1 = clamp_stages((RP == 16 ? 40 : RP == 32 ? 64 : 72) * 1024 / STAGE1);
+    static constexpr int S1 = clamp_stages((RP == 16 ? 40 : RP == 32 ? 64 : RP == 64 ? 84 : 110) * 1024 / STAGE1);
     static constexpr int PART = APPLY_WARPS * 16 * RP * 4;          // the warps' sums, in the place of the stages
     static constexpr int SMEM1 = larger(PART, S1 * STAGE1);
 
-    static constexpr int UNITS = RP * SIZE >= 128 ? 4 : 8;
+    static constexpr int UNITS = RP * SIZE >= 128 ? 4 : 8;          // FP32, rank 16, 1024 tokens, 1024 x 1024: eight 8.8 us, four 9.5
     static constexpr int COLUMNS = UNITS * 32;
     static constexpr int Y_PIECES = COLUMNS * SIZE / 16, B_PIECES = RP * SIZE / 16;   // 16-byte pieces of a row of y, of B
     static constexpr int Y_BYTES = M * Y_PIECES * 16;
     static constexpr int STAGE2 = Y_BYTES + COLUMNS * B_PIECES * 16;
-    static constexpr int S2 = clamp_stages((RP == 16 ? 48 : RP == 32 ? 64 : RP == 64 ? 84 : WIDE ? 144 : 72) * 1024 / STAGE2);
+    static_assert(M * Y_PIECES >= APPLY_THREADS && SUBS * M * 8 >= APPLY_THREADS, "a copy of x and of y for every thread");
+    static constexpr int S2 = clamp_stages((RP == 16 ? 48 : RP == 32 ? 72 : RP == 64 ? 84 : 110) * 1024 / STAGE2);
     static constexpr int PER_SM = RP == 16 ? 4 : RP == 32 ? 3 : 2;  // blocks an SM has room for: small ranks leave room for more, and
                                                                     // each of them has little in flight (4096 tokens of rank 16: four
                                                                     // 21.8 us, three 25.8, two 27.3)
@@ -628,10 +636,11 @@ __global__ void __launch_bounds__(APPLY_THREADS, ApplyShape<T, RP>::PER_SM) adap
 
 // ---- 16-bit types, tiles of 128 rows: tcgen05 ------------------------------------------------------
 // The same two kernels with the 128 rows on the M side of tcgen05.mma and sums in tensor memory: one thread issues a stage's MMAs,
-// so the warps' work is copies and the last step alone (16384 tokens of rank 64, 4096 x 10240: 180 us, where tiles of 16 rows and
-// mma.sync, whose ldmatrix and accumulators keep the SMs busier than the memory, take 265).  Stages are rows of 128 bytes, 16-byte pieces exchanged within
-// eight rows, which is both what cp.async writes without conflicts and the 128-byte swizzle that the MMAs read.  Rows that are not
-// there are left as they are: a row of A only makes its own row of D.
+// so the warps' work is copies and the last step alone (16384 tokens of rank 64, 4096 x 10240: 182 us, where tiles of 16 rows and
+// mma.sync, whose ldmatrix and accumulators keep the SMs busier than the memory, take 265; the bytes are 129 us at the copy
+// rate).  Stages are rows of 128 bytes, 16-byte pieces exchanged within eight rows, which is both what cp.async writes without
+// conflicts and the 128-byte swizzle that the MMAs read.  Rows of a tile that are not there are not copied: whatever stands in their
+// place only makes their own rows of the sums.
 constexpr int TC_ROWS = MANY;
 
 template <int RP>
@@ -647,7 +656,8 @@ struct TcShape {
     static constexpr int SMEM2 = S2 * STAGE2 + 1024;
     static constexpr int PER_SM1 = 2, PER_SM2 = RP == 128 ? 2 : 3;  // blocks an SM has room for
     // Columns of tensor memory: sums, and in the second kernel A x, two values to a column, first parts and second parts.
-    static constexpr uint32_t TMEM1 = RP < 32 ? 32 : RP, TMEM2 = COLUMNS + RP <= 128 ? 128 : 256;
+    static constexpr uint32_t TMEM1 = RP, TMEM2 = COLUMNS + RP <= 128 ? 128 : 256;
+    static_assert(RP >= 32, "the least that can be allocated");
 };
 
 template <typename T>
@@ -764,20 +774,18 @@ __global__ void __launch_bounds__(APPLY_THREADS) adapter_down_tc_kernel(const Ap
         ok = __syncthreads_and(ok);
         tc_fence_after();
         if (ok) {
-            // lanes of tensor memory are rows; four warps have 32 each, the other four (RP > 16) the second half of the columns
-            constexpr int WIDTH = RP > 16 ? RP / 2 : 16;
+            // lanes of tensor memory are rows; four warps have 32 each, the other four the second half of the columns
+            constexpr int WIDTH = RP / 2;
             const int row = (warp & 3) * 32 + lane, half = warp >> 2;
-            if (RP > 16 || half == 0) {
-                float* to = p.sums + ((size_t)(share * p.tile_count + tile_index) * TC_ROWS + row) * RP + half * WIDTH;
+            float* to = p.sums + ((size_t)(share * p.tile_count + tile_index) * TC_ROWS + row) * RP + half * WIDTH;
 #pragma unroll
-                for (int c = 0; c < WIDTH; c += 16) {
-                    uint32_t v[16];
-                    tmem_ld16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * WIDTH + c, v);
-                    tmem_ld_wait();
-                    if (row < tile.z)
+            for (int c = 0; c < WIDTH; c += 16) {
+                uint32_t v[16];
+                tmem_ld16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * WIDTH + c, v);
+                tmem_ld_wait();
+                if (row < tile.z)
 #pragma unroll
-                        for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(to + c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                }
+                    for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(to + c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
             }
         } else if (tid == 0 && p.status) {
             atomicOr(p.status, STATUS_WAIT_TIMEOUT);
@@ -878,7 +886,7 @@ __global__ void __launch_bounds__(APPLY_THREADS, TcShape<RP>::PER_SM2) adapter_u
     {
         constexpr int PART_ROWS = RP == 128 ? 32 : 64, PITCH = RP * 2 + 16;     // rows at a time, and bytes of a row
         static_assert(2 * PART_ROWS * PITCH <= S::STAGE2, "both parts fit into a slot");
-        constexpr int LANES = RP / 4, ROWS = APPLY_THREADS / LANES, PASSES = PART_ROWS / ROWS, TOGETHER = PASSES <= 1 ? 4 : 2;
+        constexpr int LANES = RP / 4, ROWS = APPLY_THREADS / LANES, PASSES = PART_ROWS / ROWS;
         char* const staged = ring_ptr + (S::S2 - 1) * S::STAGE2;
         const int col = tid % LANES * 4, r0 = tid / LANES;
         const size_t stride = (size_t)p.tile_count * (TC_ROWS * RP);
@@ -889,7 +897,7 @@ __global__ void __launch_bounds__(APPLY_THREADS, TcShape<RP>::PER_SM2) adapter_u
             float4 v[PASSES];
 #pragma unroll
             for (int i = 0; i < PASSES; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll TOGETHER
+#pragma unroll 2
             for (int q = 0; q < p.k_split; ++q) {
 #pragma unroll
                 for (int i = 0; i < PASSES; ++i) {
@@ -1051,7 +1059,7 @@ int launch_many(ApplyArgs a, cudaStream_t stream) {
 
 template <typename T, int RP>
 int launch_apply_rank(const ApplyArgs& a, bool many, bool fast, cudaStream_t stream) {
-    if constexpr (sizeof(T) == 2)
+    if constexpr (sizeof(T) == 2 && RP > 16)
         if (many) return fast ? launch_many<T, RP, true>(a, stream) : launch_many<T, RP, false>(a, stream);
     return fast ? launch_few<T, RP, true>(a, stream) : launch_few<T, RP, false>(a, stream);
 }

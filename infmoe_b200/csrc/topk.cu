@@ -1,5 +1,12 @@
 // Routing to the k best experts, and token rows to k experts and back.  The reference routes to one expert (top-k is a TODO
 // there); these kernels stand beside its select / scatter / gather (plugin/cuda/moe.cu:147-258) for layers that route to k.
+//
+//   select   s = softmax(l) or sigmoid(l), c = s + bias; the k best c of the best groups, weights s / sum s of these.  65536 tokens,
+//            8 of 256 experts in groups, FP32: 59 us, 5.4 times what its 71 MB take at the copy rate; bound by instructions (591
+//            a token, the integer pipe 64 % busy).  Few tokens: 3 us.
+//   scatter  routed[j] = x[pos[j] / k].  32768 rows of 8 KB: 55 to 57 us, 1.25 times its 287 MB; writes.
+//   combine  out[t] = sum_s w[t, s] y[row(t, s)] + (1 - sum_s w[t, s]) x[t].  4096 tokens x 4 rows of 16 KB and their own: 62 us, its
+//            389 MB at 6.3 TB/s.
 #include <cfloat>
 #include <type_traits>
 
