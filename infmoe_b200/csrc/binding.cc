@@ -161,8 +161,7 @@ PyObject* select_topk(PyObject* const* a) {
     const Rows rows = rows_of(logits, cfg->expert_count, "logits");
     const int dtype = dtype_code(logits);
     const at::Device device = logits.device();
-    if (bias.defined() && bias.device() != device)
-        refuse("logits are on %s, the router's bias on %s", device.str().c_str(), bias.device().str().c_str());
+    if (bias.defined()) check_array(bias, {cfg->expert_count}, at::kFloat, device, "the router's bias");
     if (status.defined()) check_array(status, {1}, at::kInt, device, "status");
     const auto shape = with_last(logits, cfg->top_k);
     const at::Tensor gate = output(a[3], shape, at::kInt, device, "gate"), weight = output(a[4], shape, at::kFloat, device, "weight");

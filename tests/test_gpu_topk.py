@@ -170,6 +170,16 @@ def test_select_bias_is_read_at_every_call():
     assert (router.select(l)[0] == 3).all() and not (first == 3).all()
 
 
+def test_select_refuses_a_bias_that_was_replaced():
+    l = logits_of(30, 16, torch.float32, 9)
+    router = TopKRouter(16, 1, score="sigmoid", bias=torch.zeros(16, device="cuda"))
+    for bias in (torch.zeros(15, device="cuda"), torch.zeros(16, dtype=torch.bfloat16, device="cuda"),
+                 torch.zeros(32, device="cuda")[::2], torch.zeros(16)):
+        router.bias = bias
+        with pytest.raises(ValueError, match="bias"):
+            router.select(l)
+
+
 def slots_of(T, k, E, none=0.1, seed=0):
     rng = np.random.default_rng(seed)
     gate = np.stack([rng.permutation(E)[:k] for _ in range(T)]).astype(np.int32) if T else np.zeros((0, k), np.int32)
