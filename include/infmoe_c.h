@@ -151,7 +151,8 @@ INFMOE_API int infmoe_layer_expert_forward_scatter(infmoe_layer* layer, const fl
  * expert gate[t][s] (T5_FF: E(x) = x + f(x), so x[t] + sum_s weight[t][s] * f_s(x[t])).  d_gate [token_num][top_k] and
  * d_weight [token_num][top_k] come from infmoe_expert_select_topk; a gate outside [0, expert_count) is a place without an
  * expert, and a token without any passes unchanged.  Experts resident, streamed or of a registered sublayer as in
- * infmoe_layer_enqueue; the variant's own routing and output mix play no part.  No counterpart in the reference (top-1). */
+ * infmoe_layer_enqueue; the variant's own routing and output mix play no part, and
+ * infmoe_layer_last_routing stays that of the last enqueue.  No counterpart in the reference (top-1). */
 INFMOE_API int infmoe_layer_topk_workspace_bytes(const infmoe_layer* layer, int64_t token_num, int32_t top_k, size_t* bytes);
 INFMOE_API int infmoe_layer_forward_topk(infmoe_layer* layer, const float* d_input, const int32_t* d_gate,
                                          const float* d_weight, int64_t token_num, int32_t top_k, float* d_output,

@@ -5,7 +5,7 @@
     out = adapters.apply(x, y, plan)                 # y + scale * b (a x), row by row with the row's adapter
 
 A plan holds for every projection of the batch whose set has as many adapters.  `MoELayer.forward(x, adapters=..., plan=...)`
-adds the adapters of a layer's requests to its output.
+adds the adapters of a layer's requests to its output.  For inference: results carry no gradient.
 """
 from __future__ import annotations
 

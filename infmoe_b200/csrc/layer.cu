@@ -1019,7 +1019,7 @@ int infmoe_layer_workspace_bytes(const infmoe_layer* L, int64_t T, size_t* bytes
 // routing happened on the rank that owns the token.
 // region_count / region_size (expert-parallel receive buffer): the T rows are slots in regions of region_size, of
 // which only the first region_count[s] of region s hold a row.
-// some_without: a gate outside [0, E) is a row without an expert and no error.
+// some_without (top-k passes): a gate outside [0, E) is a row without an expert and no error; infmoe_layer_last_routing stays.
 static int layer_run(infmoe_layer* L, const float* d_in, float* d_out, void* d_ws, size_t ws_bytes, int64_t T,
                      void* stream_v, const int* given_gate, const float* row_score = nullptr,
                      const unsigned long long* row_dst = nullptr, const int* region_count = nullptr,
@@ -1086,11 +1086,13 @@ static int layer_run(infmoe_layer* L, const float* d_in, float* d_out, void* d_w
     buf.part_count = (int*)(base + w.part_count);
     const int* gate_in = given_gate ? given_gate : gate;
     if (given_gate) score = const_cast<float*>(row_score);   // scores of the caller's rows, or none
-    L->last_gate = gate_in;
-    L->last_score = score;
-    L->last_pos = pos;
-    L->last_count = count;
-    L->last_offset = offset;
+    if (!some_without) {     // rows of a top-k pass are not its tokens, and its workspace may be gone after the call
+        L->last_gate = gate_in;
+        L->last_score = score;
+        L->last_pos = pos;
+        L->last_count = count;
+        L->last_offset = offset;
+    }
 
     INFMOE_TRY(prof_mark(L, 0, stream));
     // 1. routing (plugin/MoELayerPlugin.cc:312-345)

@@ -10,6 +10,7 @@
 every token to one expert (top-k is a TODO there).
 
 All functions work on torch's current stream of the tensors' device, and allocate what they return unless they are given it.
+They are for inference: what they return carries no gradient.
 """
 from __future__ import annotations
 

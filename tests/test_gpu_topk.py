@@ -334,6 +334,23 @@ def test_layer_of_identity_experts():
     assert torch.allclose(layer.forward_topk(dx, gate, weight), dx, rtol=1e-6, atol=1e-6)
 
 
+@pytest.mark.parametrize("mode", ["enqueue_first", "topk_first"])
+def test_last_routing_is_that_of_the_last_enqueue(mode):
+    layer, _, x = small_layer(4, 32, 64)
+    dx = torch.from_numpy(x).cuda()
+    gate, weight = TopKRouter(4, 2).select(logits_of(70, 4, torch.float32))
+    if mode == "topk_first":
+        layer.forward_topk(dx, gate, weight)
+        with pytest.raises(capi.InfMoEError):
+            layer.last_routing()
+    layer.forward(dx)
+    before = layer.last_routing()
+    layer.forward_topk(dx, gate, weight)
+    assert layer.last_routing() == before and gate.data_ptr() not in before
+    layer.sync_status()
+    layer.terminate()
+
+
 def test_router_rows_and_experts_together(oracle):
     """Router -> dispatch -> rows to experts -> experts of the caller -> rows back, against the layer's own pass and 64 bits."""
     E, D, F, k, T = 8, 128, 256, 3, 70
