@@ -1,6 +1,6 @@
 // The Python module infmoe_b200._binding: checks of arguments, outputs and calls of the operators on torch tensors that stand in
 // topk.py and adapters.py.  Through ctypes, torch.empty and shapes read in Python a call took 12 to 13 us of host time, here it
-// takes 3.5 to 4.7: what bounds a small batch, whose kernels take 2 to 3.  Everything else goes through ctypes (capi.py).
+// takes 3.5 to 4.7 (4 to 9 on a slower host): what bounds a small batch, whose kernels take 2 to 3.  Everything else goes through ctypes (capi.py).
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
