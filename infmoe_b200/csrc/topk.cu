@@ -2,7 +2,7 @@
 // there); these kernels stand beside its select / scatter / gather (plugin/cuda/moe.cu:147-258) for layers that route to k.
 //
 //   select   s = softmax(l) or sigmoid(l), c = s + bias; the k best c of the best groups, weights s / sum s of these.  65536 tokens,
-//            8 of 256 experts in groups, FP32: 59 us, 5.4 times what its 71 MB take at the copy rate; bound by instructions (591
+//            8 of 256 experts in groups, FP32: 59 us, 5.4 times what its 71 MB take at the copy rate; bound by instructions (567
 //            a token, the integer pipe 64 % busy).  Few tokens: 3 us.
 //   scatter  routed[j] = x[pos[j] / k].  32768 rows of 8 KB: 55 to 57 us, 1.25 times its 287 MB; writes.
 //   combine  out[t] = sum_s w[t, s] y[row(t, s)] + (1 - sum_s w[t, s]) x[t].  4096 tokens x 4 rows of 16 KB and their own: 62 us, its
@@ -138,7 +138,7 @@ __device__ __noinline__ int select_in_64_bits(const SelectArgs& a, long long t, 
 // bits nothing moves at all: their FP32 form has 13 bits to spare, which hold the whole index.  A lane sorts its keys (two
 // instructions a comparison), and each round takes the largest of the 32 heads by one redux and moves that lane's list on.  Lists
 // hold four or five keys; a lane that has more and uses up its list shows a last one that nothing exceeds, which counts as undecided
-// (65536 tokens, 8 of 256 experts, of which 16 lanes hold what four of eight groups have: 0.4 % with lists of four).
+// (65536 tokens, 8 of 256 experts, of which 16 lanes hold what four of eight groups have: 277 undecided with lists of four, 149 of five).
 template <int V>
 struct Keys {
     static constexpr int PLACE_BITS = V <= 1 ? 0 : V <= 2 ? 1 : V <= 4 ? 2 : V <= 8 ? 3 : V <= 16 ? 4 : 5;
@@ -409,7 +409,8 @@ __device__ __forceinline__ void load_logits(const SelectArgs& a, long long t, in
 // A warp per token, tokens a grid apart, 32 to a warp before the block meets.  As many tokens as fit into the lanes (four with 5 to
 // 8 experts each) then get their weights together: by token that took 10 of 45 us (65536 tokens, 8 of 256 experts).  Tokens
 // that 32 bits leave undecided wait until the block's are done, and its warps share them; in the loop itself that choice cost every
-// token its registers, 20 us, and by each warp after a few tokens 4 us more than so.
+// token its registers, 20 us, and by each warp after a few tokens 4 us more than so.  Of 59 us the undecided 149 take 9 (5 to 14 more
+// by all threads of a block, an expert to each).
 template <typename T, int V, ChosenBy BY>
 __global__ void __launch_bounds__(SELECT_WARPS * 32, V <= 8 ? 4 : V <= 16 ? 3 : 2) select_topk_kernel(const __grid_constant__ SelectArgs a) {
     __shared__ uint2 s_found[SELECT_WARPS][MAX_ROUNDS];

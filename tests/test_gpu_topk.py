@@ -100,6 +100,35 @@ def test_select_where_32_bits_do_not_tell_apart(score):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("score,bias", [("softmax", False), ("softmax", True), ("sigmoid", False), ("sigmoid", True)])
+@pytest.mark.parametrize("E,groups,top_groups", [(20, 1, 1), (31, 1, 1), (96, 8, 6), (160, 8, 5), (256, 8, 4), (270, 30, 20), (513, 1, 1),
+                                                 (544, 17, 4), (1000, 1, 1), (1024, 32, 3)])
+def test_select_alone_as_among_others(E, groups, top_groups, score, bias, dtype):
+    """More than 16 experts to a token are always chosen in 64 bits: a token's choice does not depend on those beside it."""
+    t = TYPES[dtype]
+    rng = np.random.default_rng(E + groups)
+    l = logits_of(48, E, t, E)
+    l[1] = -np.inf
+    l[2, : E // 2] = torch.finfo(t).min
+    l[3, ::2] = np.nan
+    l[4] = l[4, 0].item()                                # all alike
+    l[5, E // 3] = np.inf
+    l[6, 3:] = -np.inf                                   # fewer than k
+    l[7] = torch.from_numpy(rng.integers(0, 3, size=E)).to(t).cuda()
+    b = torch.from_numpy(np.round(rng.standard_normal(E), 1).astype(np.float32) * 0.1).cuda() if bias else None
+    if bias:
+        b[0], b[E - 1] = -np.inf, np.nan
+    for best in (1, 2) if groups > 1 else (1,):
+        for renormalise in (True, False):
+            gate, weight = check_select(l, 20, score, b, groups, top_groups, best, renormalise)
+            for i in range(9):
+                one = check_select(l[i:i + 1], 20, score, b, groups, top_groups, best, renormalise)
+                assert torch.equal(one[0][0], gate[i]) and torch.equal(one[1][0], weight[i])
+                two = check_select(l[i:i + 2], 20, score, b, groups, top_groups, best, renormalise)
+                assert torch.equal(two[0], gate[i:i + 2]) and torch.equal(two[1], weight[i:i + 2])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_select_masks(score, dtype):
     t = TYPES[dtype]
