@@ -279,7 +279,7 @@ __device__ __forceinline__ bool select_in_32_bits(const SelectArgs& a, const flo
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) key[j] = (key_of(l[j]) & ~LOW) | (low0 - j);
+        for (int j = 0; j < V; ++j) key[j] = (key_of(l[j] + 0.f) & ~LOW) | (low0 - j);     // -0 is 0
     }
     uint32_t head[K::DEPTH];
     largest<V, K::DEPTH>(key, head);

@@ -81,6 +81,27 @@ def test_select_ties_go_to_the_lowest_index(dtype, score):
 
 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("E,groups,top_groups", [(2, 1, 1), (24, 4, 2), (60, 5, 3), (100, 10, 3), (256, 8, 4), (513, 1, 1), (1024, 32, 3)])
+def test_select_zeros_of_both_signs_are_ties(E, groups, top_groups, dtype, score):
+    """A logit masked by a product with zero is +0 or -0: one value.  16 experts are chosen in 32 bits, 17 in 64."""
+    rng = np.random.default_rng(E)
+    l = np.where(rng.random((60, E)) < 0.8, np.copysign(0.0, rng.standard_normal((60, E))), -1.0)
+    l[0], l[0, -1] = -0.0, 0.0
+    l[1:20] = np.where(rng.random((19, E)) < 0.2, 1.0, l[1:20])
+    l = torch.from_numpy(l).cuda().to(TYPES[dtype])
+    assert torch.signbit(l[0, 0]) and not torch.signbit(l[0, -1])
+    size = E // groups
+    for k in (1, 2, 16, 17):
+        for best in (1, 2):
+            if k <= E and best == 1:
+                check_select(l, k, score)
+                check_select(l, k, score, torch.full((E,), -0.0, device="cuda"))
+            if groups > 1 and k <= top_groups * size:
+                check_select(l, k, score, None, groups, top_groups, best)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_select_where_32_bits_do_not_tell_apart(score):
     """Scores plus bias that differ by less than a 32-bit sum shows: the choice is that of 64 bits."""
     rng = np.random.default_rng(5)
