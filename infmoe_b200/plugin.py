@@ -318,7 +318,9 @@ class MoELayer:
         self.enqueue(x.data_ptr(), out.data_ptr(), self._ws.data_ptr(), self._ws.numel(), T, s)
         if adapters is not None:
             if stream is not None:
-                with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=x.device)):
+                # 0 is the default stream, of which ExternalStream makes another one
+                on = torch.cuda.ExternalStream(stream, device=x.device) if stream else torch.cuda.default_stream(x.device)
+                with torch.cuda.stream(on):
                     return adapters.apply(x, out, plan, out=out)
             adapters.apply(x, out, plan, out=out)
         return out

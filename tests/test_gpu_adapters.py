@@ -378,3 +378,38 @@ def test_rows_past_32_bits():
     into = x[:, 2000:2000 + d]                                      # rows apart on the way out too
     adapters.apply(x[:, :d], y, plan, out=into)
     assert torch.equal(into, got)
+
+
+@pytest.mark.parametrize("which", ["default", "side"])
+def test_layer_with_adapters_on_a_given_stream(which):
+    """The adapters run on the stream that the layer was given; 0 is the handle of the default one."""
+    from tests.test_gpu_topk import small_layer
+
+    layer, _, xs = small_layer(4, 64, 128, on_device=True)
+    rng = np.random.default_rng(1)
+    x = torch.from_numpy(xs).cuda()
+    f = lambda *s: torch.from_numpy(rng.standard_normal(s).astype(np.float32) * 0.1).cuda()  # noqa: E731
+    adapters = Adapters(f(3, 8, 64), f(3, 64, 8), scale=2.0)
+    plan = adapters.plan(torch.from_numpy(owners(rng, 70, 3, 6)).cuda())
+    want = adapters.apply(x, layer.forward(x), plan)
+    stream = torch.cuda.default_stream() if which == "default" else torch.cuda.Stream()
+    assert (stream.cuda_stream == 0) == (which == "default")
+    seen = []
+
+    class Recorded:
+        def apply(self, *args, **kw):
+            seen.append(torch.cuda.current_stream(x.device).cuda_stream)
+            return adapters.apply(*args, **kw)
+
+    torch.cuda.synchronize()
+    for _ in range(3):
+        out = torch.full_like(x, 7.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            torch.cuda._sleep(20_000_000)           # about 10 ms: adapters on another stream would not wait for the layer's pass
+        got = layer.forward(x, stream=stream.cuda_stream, out=out, adapters=Recorded(), plan=plan)
+        assert got is out
+        stream.synchronize()
+        assert torch.equal(out, want)
+    assert seen == [stream.cuda_stream] * 3
+    layer.terminate()
