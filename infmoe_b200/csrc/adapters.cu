@@ -190,11 +190,19 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
 }
 
 // An FP32 value as two of 11 significant bits: cut off behind the eleventh, and what is left of it, rounded.  2^-22 of the value is
-// left out at most.  An infinity has no second part.
+// left out at most.  An infinity has no second part; times a zero second
+// part it is NaN.
 __device__ __forceinline__ void split_tf32(const uint32_t v, uint32_t& hi, uint32_t& lo) {
     hi = v & 0xffffe000u;
     const float rest = __fsub_rn(__uint_as_float(v), __uint_as_float(hi));      // NaN for NaN
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"((v & 0x7fffffffu) == 0x7f800000u ? 0.f : rest));
+}
+// sum_i a[i] b[i] in FP32: stands in the place of a sum of parts that is no finite number.
+__device__ __forceinline__ float plain_sum(const float* a, const float* b, int n) {
+    float sum = 0.f;
+#pragma unroll 1
+    for (int i = 0; i < n && sum == sum; ++i) sum = fmaf(a[i], b[i], sum);
+    return sum;
 }
 
 // What is left of v after its rounding to T (0 where that is no finite value).
@@ -394,6 +402,16 @@ __global__ void __launch_bounds__(APPLY_THREADS, ApplyShape<T, RP>::PER_SM) adap
         for (int g = 1; g < APPLY_WARPS; ++g) {
             const float4 o = *reinterpret_cast<const float4*>(part + g * M * RP + i);
             sum = make_float4(sum.x + o.x, sum.y + o.y, sum.z + o.z, sum.w + o.w);
+        }
+        if constexpr (WIDE) {
+            const int from = stage_begin * S::K_CHUNK, n = min(p.d_in - from, stages * S::K_CHUNK);
+            const T* const x = static_cast<const T*>(p.x) + s_pos[i / RP] * p.ldx + from;
+            const T* const w = A + (long long)(i % RP) * p.d_in + from;
+            const int left = rank - i % RP;
+            if (!(fabsf(sum.x) <= FLT_MAX) && 0 < left) sum.x = plain_sum(x, w, n);
+            if (!(fabsf(sum.y) <= FLT_MAX) && 1 < left) sum.y = plain_sum(x, w + p.d_in, n);
+            if (!(fabsf(sum.z) <= FLT_MAX) && 2 < left) sum.z = plain_sum(x, w + 2ll * p.d_in, n);
+            if (!(fabsf(sum.w) <= FLT_MAX) && 3 < left) sum.w = plain_sum(x, w + 3ll * p.d_in, n);
         }
         *reinterpret_cast<float4*>(sums + i) = sum;
     }
@@ -605,6 +623,19 @@ __global__ void __launch_bounds__(APPLY_THREADS, ApplyShape<T, RP>::PER_SM) adap
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 if (!row_ok[h]) continue;
+                if constexpr (WIDE) {
+                    float all = 0.f;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) all += fabsf(sum[k / 2][2 * h + (k & 1)]);
+                    if (!(all <= FLT_MAX))
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            float& o = sum[k / 2][2 * h + (k & 1)];
+                            if (!(fabsf(o) <= FLT_MAX) && k < left)
+                                o = plain_sum(reinterpret_cast<const float*>(v_smem + (g + 8 * h) * S::V_ROW),
+                                              reinterpret_cast<const float*>(B) + (long long)(p.d_out - left + k) * p.rank, rank);
+                        }
+                }
 #pragma unroll
                 for (int i = 0; i < 8 / N; ++i) {
                     uint4* const at = reinterpret_cast<uint4*>(smem + slot + cell[h][i]);

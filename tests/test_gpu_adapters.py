@@ -413,3 +413,67 @@ def test_layer_with_adapters_on_a_given_stream(which):
         assert torch.equal(out, want)
     assert seen == [stream.cuda_stream] * 3
     layer.terminate()
+
+
+# FP32 products are made of two parts of 11 bits to each number.  Of a number u in [1, 2) the first part leaves at most 2^-11, in
+# steps of 2^-23, and the second keeps 11 bits of that: at most 2^-23 of u is lost.  The product of the second parts, at most 2^-22, is
+# left out.  So a product of two is off by (2 + 1 + 1) 2^-23, and by one more for a sum in 32 bits that is cut off and not rounded; A x
+# and B v are one such product each where d_in and the rank are one.
+FP32_PRODUCTS_TOL = 10 * 2.0 ** -23 * (1 + 2.0 ** -8)
+
+
+def one_by_one(x, a, b, at):
+    """Adapters with one product to A x and one to B v: what they give and what 64 bits do."""
+    t = lambda v: torch.from_numpy(v.astype(np.float32)).cuda()  # noqa: E731
+    adapters = Adapters(t(a).view(-1, 1, 1), t(b).unsqueeze(2))
+    y = torch.zeros(len(x), b.shape[1], device="cuda")
+    got = adapters.apply(t(x).view(-1, 1), y, adapters.plan(torch.from_numpy(at).cuda()))
+    with np.errstate(invalid="ignore"):
+        return got.double().cpu().numpy(), (x * a[at])[:, None] * b[at]
+
+
+def test_fp32_infinities_and_the_largest_numbers():
+    """What the formula makes of them: an infinity stays one where the other factor is exact in few bits, and is NaN only where it
+    meets a zero or its opposite."""
+    big = np.float64(np.finfo(np.float32).max)
+    x = np.array([np.inf, -np.inf, np.nan, big, -big, big * (1 - 2.0 ** -12), 1.0, 3.0, 0.0, 1 + 2.0 ** -23] * 4).astype(np.float32).astype(np.float64)
+    a = np.array([1.0, 2.0 ** -20, -0.75, 2.0 ** -20 * (1 + 2.0 ** -12 + 2.0 ** -23)])
+    b = np.array([[1.0, -2.0, 0.5, 1 / 3, 0.0, 2.0 ** -30]] * 4).astype(np.float32).astype(np.float64)
+    at = np.repeat(np.arange(4), 10).astype(np.int32)
+    got, want = one_by_one(x, a, b, at)
+    some = np.abs(want) <= big
+    beyond = ~some & ~np.isnan(want)
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+    np.testing.assert_array_equal(got[beyond], np.sign(want[beyond]) * np.inf)
+    assert (np.abs(got[some] - want[some]) <= FP32_PRODUCTS_TOL * np.abs(want[some])).all()
+    # infinite weights
+    got, want = one_by_one(np.array([1.0, -2.0, 0.0]), np.array([np.inf]), np.array([[1.0, -1.0]]), np.zeros(3, np.int32))
+    assert (got[:2] == want[:2]).all() and np.isnan(got[2]).all()
+    got, want = one_by_one(np.array([1.0, -2.0, 0.0]), np.array([1.0]), np.array([[np.inf, -np.inf, 4.0]]), np.zeros(3, np.int32))
+    np.testing.assert_array_equal(got, np.where(np.isnan(want), np.nan, want))
+
+
+@pytest.mark.parametrize("r", [3, 16, 24, 64, 128])
+def test_fp32_rows_beside_infinities_keep_their_bits(r):
+    """A row's result does not depend on what the other rows of its tile hold, nor on what lies in memory past the tile and the rank."""
+    rng = np.random.default_rng(r)
+    T, n, d_in, d_out = 61, 2, 300, 140
+    f = lambda *s: torch.from_numpy(rng.standard_normal(s).astype(np.float32)).cuda()  # noqa: E731
+    x, y, a, b = f(T, d_in), f(T, d_out), f(n, r, d_in), f(n, d_out, r)
+    at = owners(rng, T, n, 4)
+    adapters = Adapters(a, b)
+    plan = adapters.plan(torch.from_numpy(at).cuda())
+    want = adapters.apply(x, y, plan)
+    odd = x.clone()
+    odd[3::7, 5], odd[4::7, 200], odd[5::7, 299] = np.inf, torch.finfo(torch.float32).max, np.nan
+    got = adapters.apply(odd, y, plan)
+    same = np.array([t % 7 not in (3, 4, 5) or not 0 <= at[t] < n for t in range(T)])
+    assert torch.equal(got[same], want[same]) and not torch.isfinite(got[5::7][(at[5::7] >= 0) & (at[5::7] < n)]).any()
+    # an infinite column of one adapter's A x, B's row of one column of out
+    a[0, r // 2, 7] = np.inf
+    b[1, 100] = np.nan
+    got = adapters.apply(x, y, plan)
+    two = at == 1
+    keep = np.arange(d_out) != 100
+    assert torch.equal(got[two][:, keep], want[two][:, keep]) and torch.isnan(got[two][:, 100]).all()
+    assert not torch.isfinite(got[at == 0]).any()
