@@ -413,7 +413,8 @@ INFMOE_API int infmoe_t5ff_run_static(int64_t rows, int32_t embedding_size, int3
 /* ------------------------------------------------------------------------ */
 /* No counterparts in the reference (top-k routing is a TODO there).  Unlike the
  * functions above these take FP32, FP16 or BF16 elements; all of them compute in
- * FP32 or more and round once, when they store. */
+ * FP32 or more and round once, when they store.  FP32 adapters form a product from
+ * two parts of 11 bits to each factor: off by at most 2^-21 of it, to either side. */
 typedef enum infmoe_dtype { INFMOE_F32 = 0, INFMOE_F16 = 1, INFMOE_BF16 = 2 } infmoe_dtype;
 typedef enum infmoe_score { INFMOE_SCORE_SOFTMAX = 0, INFMOE_SCORE_SIGMOID = 1 } infmoe_score;
 

@@ -189,13 +189,15 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// An FP32 value as two of 11 significant bits: cut off behind the eleventh, and what is left of it, rounded.  2^-22 of the value is
-// left out at most.  An infinity has no second part; times a zero second
-// part it is NaN.
+// An FP32 value as two of 11 significant bits: rounded to the first, and what that leaves rounded to the second.  Of a value in [1, 2) the
+// first leaves at most 2^-11 in steps of 2^-23, so at most 2^-23 is lost.  The product of two second parts, at most 2^-22 of the whole, is left
+// out: a product is off by at most 2^-21, to either side (a first part that is cut off made it 2^-20 and always too small).  With that product
+// rank 32 takes 131 us for 119 and the error of sums of 4 to 4096 terms is the same within 10 %: it is that of sums in the tensor cores' 32 bits.
+// An infinity, NaN, and what the first part rounds to an infinity have no such parts: the second is NaN or the opposite infinity, and
+// every sum that it enters is NaN (plain_sum).
 __device__ __forceinline__ void split_tf32(const uint32_t v, uint32_t& hi, uint32_t& lo) {
-    hi = v & 0xffffe000u;
-    const float rest = __fsub_rn(__uint_as_float(v), __uint_as_float(hi));      // NaN for NaN
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"((v & 0x7fffffffu) == 0x7f800000u ? 0.f : rest));
+    hi = (v + 0x1000u) & 0xffffe000u;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(__fsub_rn(__uint_as_float(v), __uint_as_float(hi))));
 }
 // sum_i a[i] b[i] in FP32: stands in the place of a sum of parts that is no finite number.
 __device__ __forceinline__ float plain_sum(const float* a, const float* b, int n) {

@@ -432,6 +432,21 @@ def one_by_one(x, a, b, at):
         return got.double().cpu().numpy(), (x * a[at])[:, None] * b[at]
 
 
+def test_fp32_products():
+    """Numbers whose last 13 bits are as large as they can be are what a first part that is cut off serves worst."""
+    rng = np.random.default_rng(17)
+    f = lambda *s: 1 + rng.integers(0, 8, s) * 2.0 ** -10 + (2.0 ** 13 - 1 - rng.integers(0, 64, s)) * 2.0 ** -23  # noqa: E731
+    at = rng.integers(0, 64, size=600).astype(np.int32)
+    for x, a, b in ((f(600), f(64), f(64, 100)), (f(600), np.ones(64), f(64, 100)),
+                    *((1 + (rng.integers(0, 1 << 23, s) * 2.0 ** -23) for s in (600, 64, (64, 100))) for _ in range(4))):
+        sign = rng.choice([-1.0, 1.0], size=64)
+        got, want = one_by_one(x, a * sign, b, at)
+        off = (got - want) / want
+        assert np.abs(off).max() <= FP32_PRODUCTS_TOL, np.abs(off).max() * 2 ** 23
+        # cutting off after each product shrinks by up to two units of 2^-23 in the mean; nothing else has a side
+        assert abs(off.mean()) <= 2 * 2.0 ** -23, off.mean() * 2 ** 23
+
+
 def test_fp32_infinities_and_the_largest_numbers():
     """What the formula makes of them: an infinity stays one where the other factor is exact in few bits, and is NaN only where it
     meets a zero or its opposite."""
