@@ -480,7 +480,8 @@ typedef struct infmoe_adapter_set {
 /* What a batch's tokens need for any number of infmoe_adapter_apply calls: the tokens grouped by adapter (in token order
  * inside each, with the kernel of infmoe_expert_count) and cut into tiles.  d_adapter_of_token [token_num]; an index outside
  * [0, adapter_count) means none.  d_plan: infmoe_adapter_plan_bytes, 16-byte aligned.  Holds for adapter sets of
- * adapter_count adapters and batches of token_num tokens. */
+ * adapter_count adapters and batches of token_num tokens.  Refused (INFMOE_ERR_UNSUPPORTED) where the tiles' rows, at most
+ * token_num + 128 (adapter_count + 1), do not fit 32 bits. */
 INFMOE_API int infmoe_adapter_plan_bytes(int64_t token_num, int32_t adapter_count, size_t* bytes);
 INFMOE_API int infmoe_adapter_plan(int64_t token_num, int32_t adapter_count, const int32_t* d_adapter_of_token, void* d_plan,
                                    size_t plan_bytes, void* stream);

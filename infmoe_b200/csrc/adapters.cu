@@ -1141,7 +1141,8 @@ int check_plan_size(const char* what, int64_t T, int32_t n) {
         set_error("%s: bad argument (T=%lld adapters=%d)", what, (long long)T, n);
         return INFMOE_ERR_INVALID_ARGUMENT;
     }
-    if (T > INT_MAX || !dispatch_supported(n)) {
+    // places in the tables of rows (adapter_rows_kernel and the products) are counted in 32 bits
+    if (T > INT_MAX || max_tiles(T, n, MANY) > INT_MAX / MANY || !dispatch_supported(n)) {
         set_error("%s: %lld tokens or %d adapters are more than a plan can hold", what, (long long)T, n);
         return INFMOE_ERR_UNSUPPORTED;
     }

@@ -182,3 +182,17 @@ def test_adapters_second_kernel_may_start_early():
         first_wait = body.index("pdl_wait()")
         assert body.index("p.sums") > first_wait and body.index("out_base + (long long)") > first_wait, kernel
         assert "mbar_wait" not in body[:first_wait]
+
+
+@pytest.mark.parametrize("n", [1, 7, 1000])
+def test_plans_of_more_rows_than_32_bits_count_are_refused(n):
+    """A plan's tiles have room for up to 128 rows each: whole tiles, and one that is not full for every adapter and for none."""
+    lib, need = capi.lib(), ctypes.c_size_t()
+    most = ((1 << 31) // 128 - (n + 1)) * 128 - 1                    # tokens whose tiles have room for 2^31 - 128 rows
+    assert lib.infmoe_adapter_plan_bytes(most, n, ctypes.byref(need)) == 0 and need.value > 12 * most
+    for T in (most + 1, (1 << 31) - 1):
+        assert lib.infmoe_adapter_plan_bytes(T, n, ctypes.byref(need)) == 6 and "plan" in capi.last_error()
+        assert lib.infmoe_adapter_plan(T, n, SOME, SOME, 1 << 60, None) == 6
+        assert _apply(T=T, adapter_count=n, ws_bytes=1 << 60) == 6
+        s = capi.AdapterSet(adapter_count=n, rank=8, d_in=32, d_out=48, dtype=2, d_a=SOME, d_b=SOME)
+        assert lib.infmoe_adapter_workspace_bytes(ctypes.byref(s), T, ctypes.byref(need)) == 6
