@@ -37,7 +37,7 @@ class Adapters:
     """A set of low-rank adapters of one projection (infmoe_adapter_set).
 
     a [n, r, d_in] and b [n, d_out, r]: contiguous CUDA tensors, float32, float16 or bfloat16 (the type of x and y too); they
-    are used in place, not copied.  scale: a number, or a float32 tensor [n].  rank: int32 tensor [n], of which adapter i uses
+    are used in place, not copied, and may be updated, or their data replaced by others of the same shape, between calls.  scale: a number, or a float32 tensor [n].  rank: int32 tensor [n], of which adapter i uses
     only the first rank[i] rows of a[i] and columns of b[i]; None: all r."""
 
     def __init__(self, a, b, scale=1.0, rank=None) -> None:
@@ -59,12 +59,11 @@ class Adapters:
         codes = {torch.float32: capi.DTYPE_F32, torch.float16: capi.DTYPE_F16, torch.bfloat16: capi.DTYPE_BF16}
         if a.dtype not in codes:
             raise ValueError(f"adapters of {a.dtype} are not supported: use float32, float16 or bfloat16")
-        self._set = capi.AdapterSet(n, r, d_in, self.d_out, codes[a.dtype], a.data_ptr(), b.data_ptr(),
-                                    scale.data_ptr() if scale is not None else None,
-                                    rank.data_ptr() if rank is not None else None)
-        self._apply = binding().apply_adapters
+        held = capi.AdapterSet(n, r, d_in, self.d_out, codes[a.dtype], a.data_ptr(), b.data_ptr(),
+                               scale.data_ptr() if scale is not None else None, rank.data_ptr() if rank is not None else None)
+        self._apply, self._set = binding().apply_adapters, bytes(held)
         # what a set can be refused for, now and not at the first call
-        capi.check(capi.lib().infmoe_adapter_workspace_bytes(ctypes.byref(self._set), 0, ctypes.byref(ctypes.c_size_t())))
+        capi.check(capi.lib().infmoe_adapter_workspace_bytes(ctypes.byref(held), 0, ctypes.byref(ctypes.c_size_t())))
 
     def plan(self, adapter_of_token) -> AdapterPlan:
         """adapter_of_token: int32 CUDA tensor, one index per token; an index outside [0, n) means none."""
@@ -74,4 +73,4 @@ class Adapters:
         """x [..., d_in], y [..., d_out] -> y plus each row's adapter of x.  out may be y (in place), not x.
 
         status (int32 [1], may be None): bit 2 is set when a bounded wait inside a kernel ran out."""
-        return self._apply(self._set, self._tensors[0], x, y, plan.buffer, plan.tokens, plan.adapter_count, out, status)
+        return self._apply(self._set, *self._tensors, x, y, plan.buffer, plan.tokens, plan.adapter_count, out, status)

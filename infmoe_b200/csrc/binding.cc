@@ -11,6 +11,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdarg>
+#include <cstring>
 #include <string>
 
 #include "infmoe_c.h"
@@ -45,6 +46,7 @@ const at::Tensor& tensor(PyObject* o, const char* what) {
     return THPVariable_Unpack(o);
 }
 at::Tensor optional(PyObject* o, const char* what) { return o == Py_None ? at::Tensor() : tensor(o, what); }
+const at::Tensor* given(PyObject* o, const char* what) { return o == Py_None ? nullptr : &tensor(o, what); }
 
 int dtype_code(const at::Tensor& t) {
     switch (t.scalar_type()) {
@@ -215,36 +217,49 @@ PyObject* combine_topk(PyObject* const* a) {
     return wrap(out);
 }
 
-// (set, a, x, y, plan buffer, plan tokens, plan adapters, out, status) -> out
-PyObject* apply_adapters(PyObject* const* a) {
-    const Held<infmoe_adapter_set> set(a[0]);
-    const at::Tensor &weights = tensor(a[1], "a"), &x = tensor(a[2], "x"), &y = tensor(a[3], "y"), &plan = tensor(a[4], "plan");
-    const long long tokens = PyLong_AsLongLong(a[5]), adapters = PyLong_AsLongLong(a[6]);
+// (bytes of the set, a, b, scale, rank, x, y, plan buffer, plan tokens, plan adapters, out, status) -> out.  Where the weights lie is asked of the
+// tensors at every call: a parameter's data may have been replaced since the set was made.
+PyObject* apply_adapters(PyObject* const* args) {
+    if (!PyBytes_Check(args[0]) || PyBytes_GET_SIZE(args[0]) != (Py_ssize_t)sizeof(infmoe_adapter_set)) refuse("not an adapter set");
+    infmoe_adapter_set set;
+    memcpy(&set, PyBytes_AS_STRING(args[0]), sizeof(set));
+    const at::Tensor &a = tensor(args[1], "a"), &b = tensor(args[2], "b"), &x = tensor(args[5], "x"), &y = tensor(args[6], "y");
+    const at::Tensor *scale = given(args[3], "scale"), *rank = given(args[4], "rank"), &plan = tensor(args[7], "plan");
+    const long long tokens = PyLong_AsLongLong(args[8]), adapters = PyLong_AsLongLong(args[9]);
     if (PyErr_Occurred()) throw Refused{};
-    const Rows rx = rows_of(x, set->d_in, "x"), ry = rows_of(y, set->d_out, "y");
-    const at::Device device = weights.device();
-    const at::ScalarType type = weights.scalar_type();
+    const Rows rx = rows_of(x, set.d_in, "x"), ry = rows_of(y, set.d_out, "y");
+    const at::Device device = a.device();
+    const at::ScalarType type = set.dtype == INFMOE_F32 ? at::kFloat : set.dtype == INFMOE_F16 ? at::kHalf : at::kBFloat16;
+    if (!a.is_cuda()) refuse("a must be a CUDA tensor");
+    check_array(a, {set.adapter_count, set.rank, set.d_in}, type, device, "a");
+    check_array(b, {set.adapter_count, set.d_out, set.rank}, type, device, "b");
+    if (scale) check_array(*scale, {set.adapter_count}, at::kFloat, device, "scale");
+    if (rank) check_array(*rank, {set.adapter_count}, at::kInt, device, "rank");
+    set.d_a = a.data_ptr();
+    set.d_b = b.data_ptr();
+    set.d_scale = scale ? (const float*)scale->data_ptr() : nullptr;
+    set.d_rank = rank ? (const int32_t*)rank->data_ptr() : nullptr;
     if (x.scalar_type() != type || y.scalar_type() != type || x.device() != device || y.device() != device)
         refuse("x and y must be %s tensors on %s, like the adapters", c10::toString(type), device.str().c_str());
-    if (rx.count != ry.count || rx.count != tokens || adapters != set->adapter_count || plan.device() != device)
+    if (rx.count != ry.count || rx.count != tokens || adapters != set.adapter_count || plan.device() != device)
         refuse("x has %lld rows, y %lld; the plan is for %lld rows and %lld adapters on %s, the set has %d on %s", (long long)rx.count,
-               (long long)ry.count, tokens, adapters, plan.device().str().c_str(), set->adapter_count, device.str().c_str());
-    const at::Tensor status = optional(a[8], "status");
+               (long long)ry.count, tokens, adapters, plan.device().str().c_str(), set.adapter_count, device.str().c_str());
+    const at::Tensor status = optional(args[11], "status");
     if (status.defined()) check_array(status, {1}, at::kInt, device, "status");
     at::Tensor out;
-    int64_t ldo = set->d_out;
-    if (a[7] == Py_None) {
+    int64_t ldo = set.d_out;
+    if (args[10] == Py_None) {
         out = at::detail::empty_cuda(y.sizes(), type, device, std::nullopt);
     } else {
-        out = tensor(a[7], "out");
-        ldo = rows_of(out, set->d_out, "out").ld;
+        out = tensor(args[10], "out");
+        ldo = rows_of(out, set.d_out, "out").ld;
         if (out.sizes() != y.sizes() || out.scalar_type() != type || out.device() != device) refuse("out must be a tensor like y");
     }
     const On on(x);
     size_t bytes = 0;
-    check(infmoe_adapter_workspace_bytes(set.get(), rx.count, &bytes));
+    check(infmoe_adapter_workspace_bytes(&set, rx.count, &bytes));
     const at::Tensor workspace = at::detail::empty_cuda({(int64_t)bytes}, at::kByte, device, std::nullopt);
-    check(infmoe_adapter_apply(set.get(), rx.count, x.data_ptr(), rx.ld, y.data_ptr(), ry.ld, out.data_ptr(), ldo, plan.data_ptr(),
+    check(infmoe_adapter_apply(&set, rx.count, x.data_ptr(), rx.ld, y.data_ptr(), ry.ld, out.data_ptr(), ldo, plan.data_ptr(),
                                workspace.data_ptr(), bytes, (int32_t*)data(status), on.stream));
     return wrap(out);
 }
@@ -253,7 +268,7 @@ PyMethodDef methods[] = {
     {"select_topk", (PyCFunction)(void (*)())Entry<select_topk>::call<6>, METH_FASTCALL, nullptr},
     {"scatter_topk", (PyCFunction)(void (*)())Entry<scatter_topk>::call<6>, METH_FASTCALL, nullptr},
     {"combine_topk", (PyCFunction)(void (*)())Entry<combine_topk>::call<6>, METH_FASTCALL, nullptr},
-    {"apply_adapters", (PyCFunction)(void (*)())Entry<apply_adapters>::call<9>, METH_FASTCALL, nullptr},
+    {"apply_adapters", (PyCFunction)(void (*)())Entry<apply_adapters>::call<12>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

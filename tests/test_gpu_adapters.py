@@ -492,3 +492,28 @@ def test_fp32_rows_beside_infinities_keep_their_bits(r):
     keep = np.arange(d_out) != 100
     assert torch.equal(got[two][:, keep], want[two][:, keep]) and torch.isnan(got[two][:, 100]).all()
     assert not torch.isfinite(got[at == 0]).any()
+
+
+def test_weights_whose_data_was_replaced():
+    """Parameters get other memory when a model is converted, moved or loaded anew: a call reads what they hold then."""
+    rng = np.random.default_rng(41)
+    n, r, d_in, d_out, T = 3, 8, 64, 72, 40
+    new = lambda: (whole(rng, (n, r, d_in), 2, torch.float32), whole(rng, (n, d_out, r), 1, torch.float32),  # noqa: E731
+                   torch.from_numpy(2.0 ** rng.integers(-3, 1, size=n).astype(np.float32)).cuda(),
+                   torch.from_numpy(rng.integers(0, r + 1, size=n).astype(np.int32)).cuda())
+    held = new()
+    x, y = whole(rng, (T, d_in), 2, torch.float32), whole(rng, (T, d_out), 9, torch.float32)
+    at = owners(rng, T, n, 4)
+    adapters = Adapters(*held)
+    plan = adapters.plan(torch.from_numpy(at).cuda())
+    kept = [t.data for t in held]                                   # the first memory stays valid
+    for _ in range(2):
+        check_exact(adapters.apply(x, y, plan), reference(x, y, *held, at), torch.float32)
+        for t, other in zip(held, new()):
+            t.data = other
+    assert [t.data_ptr() for t in held] != [t.data_ptr() for t in kept]
+    for i, other in enumerate((held[0][:, :4].contiguous(), held[1].half(), held[2][:2].contiguous(), held[3].float())):
+        good, held[i].data = held[i].data, other
+        with pytest.raises(ValueError, match="must be a contiguous"):
+            adapters.apply(x, y, plan)
+        held[i].data = good
