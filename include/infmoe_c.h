@@ -486,8 +486,8 @@ INFMOE_API int infmoe_adapter_plan_bytes(int64_t token_num, int32_t adapter_coun
 INFMOE_API int infmoe_adapter_plan(int64_t token_num, int32_t adapter_count, const int32_t* d_adapter_of_token, void* d_plan,
                                    size_t plan_bytes, void* stream);
 /* d_x [token_num][ldx], d_y [token_num][ldy], d_out [token_num][ldo], strides in elements.  d_out may be d_y (rows of
- * tokens without an adapter are then not touched), not d_x.  d_workspace: infmoe_adapter_workspace_bytes, 16-byte aligned, for
- * this call alone while it runs; a plan may serve several calls at once.  d_status (may be NULL): bit 2 is set when a bounded
+ * tokens without an adapter are then not touched), not d_x.  d_workspace: infmoe_adapter_workspace_bytes (that of a batch
+ * serves all smaller ones of the set), 16-byte aligned, for this call alone while it runs; a plan may serve several calls at once.  d_status (may be NULL): bit 2 is set when a bounded
  * wait inside a kernel ran out, and d_out is then not complete. */
 INFMOE_API int infmoe_adapter_workspace_bytes(const infmoe_adapter_set* set, int64_t token_num, size_t* bytes);
 INFMOE_API int infmoe_adapter_apply(const infmoe_adapter_set* set, int64_t token_num, const void* d_x, int64_t ldx,

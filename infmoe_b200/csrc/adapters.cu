@@ -218,6 +218,11 @@ __device__ __forceinline__ float rest_of(float v) {
 // First kernel, A x: stages of M rows of x and RP rows of A, 256 bytes of K each, so that each of the warps has a 32-byte step of K.
 // Second kernel, y + scale B v: stages of COLUMNS columns, M rows of y and COLUMNS rows of B, so that each of the warps has a unit of
 // 16 rows and 32 columns (or every other time).
+
+// Blocks an SM has room for: small ranks leave room for more, and each of them has little in flight (4096 tokens of rank 16: four
+// 21.8 us, three 25.8, two 27.3).
+constexpr int few_per_sm(int padded_rank) { return padded_rank == 16 ? 4 : padded_rank == 32 ? 3 : 2; }
+
 template <typename T, int RP>
 struct ApplyShape {
     static constexpr bool WIDE = sizeof(T) == 4;
@@ -238,9 +243,7 @@ struct ApplyShape {
     static constexpr int STAGE2 = Y_BYTES + COLUMNS * B_PIECES * 16;
     static_assert(M * Y_PIECES >= APPLY_THREADS && SUBS * M * 8 >= APPLY_THREADS, "a copy of x and of y for every thread");
     static constexpr int S2 = clamp_stages((RP == 16 ? 48 : RP == 32 ? 72 : RP == 64 ? 84 : 110) * 1024 / STAGE2);
-    static constexpr int PER_SM = RP == 16 ? 4 : RP == 32 ? 3 : 2;  // blocks an SM has room for: small ranks leave room for more, and
-                                                                    // each of them has little in flight (4096 tokens of rank 16: four
-                                                                    // 21.8 us, three 25.8, two 27.3)
+    static constexpr int PER_SM = few_per_sm(RP);
     static constexpr int V_ROW = RP * SIZE + 16;                    // bytes of a row of A x; the padding spreads rows over the banks
     static constexpr int V_BYTES = M * V_ROW;                       // 16 bits: once more for the second parts
     static constexpr int SMEM2 = S2 * STAGE2 + (WIDE ? 1 : 2) * V_BYTES;
@@ -674,7 +677,7 @@ __global__ void __launch_bounds__(APPLY_THREADS, ApplyShape<T, RP>::PER_SM) adap
 // rate).  Stages are rows of 128 bytes, 16-byte pieces exchanged within eight rows, which is both what cp.async writes without
 // conflicts and the 128-byte swizzle that the MMAs read.  Rows of a tile that are not there are not copied: whatever stands in their
 // place only makes their own rows of the sums.
-constexpr int TC_ROWS = MANY;
+constexpr int TC_ROWS = MANY, MANY_PER_SM = 2;                      // of the first kernel
 
 template <int RP>
 struct TcShape {
@@ -687,7 +690,7 @@ struct TcShape {
     static constexpr int STAGE2 = Y_BYTES + ATOMS * COLUMNS * 128;
     static constexpr int S2 = 3;
     static constexpr int SMEM2 = S2 * STAGE2 + 1024;
-    static constexpr int PER_SM1 = 2, PER_SM2 = RP == 128 ? 2 : 3;  // blocks an SM has room for
+    static constexpr int PER_SM1 = MANY_PER_SM, PER_SM2 = RP == 128 ? 2 : 3;   // blocks an SM has room for
     // Columns of tensor memory: sums, and in the second kernel A x, two values to a column, first parts and second parts.
     static constexpr uint32_t TMEM1 = RP, TMEM2 = COLUMNS + RP <= 128 ? 128 : 256;
     static_assert(RP >= 32, "the least that can be allocated");
@@ -1053,11 +1056,12 @@ __global__ void __launch_bounds__(APPLY_THREADS, TcShape<RP>::PER_SM2) adapter_u
     if (warp == 0) tmem_free(tmem, S::TMEM2);
 }
 
-constexpr int MAX_K_SPLIT = 8;
+constexpr int SMS = 148;
+constexpr int FEW_SHARES = 8, MANY_SHARES = 4;                      // of A x, at most: every block of the second kernel adds them up
 
-// Blocks to a tile: as many as run at once on 148 SMs, none with less than a stage.
+// Blocks to a tile: as many as run at once, none with less than a stage.
 int split(int tiles, int per_sm, int stages, int most) {
-    int n = 148 * per_sm / tiles;
+    int n = SMS * per_sm / tiles;
     n = n < most ? n : most;
     n = n < stages ? n : stages;
     return n > 1 ? n : 1;
@@ -1077,7 +1081,7 @@ int launch_pair(Down down, Up up, const ApplyArgs& a, size_t smem1, size_t smem2
 template <typename T, int RP, bool FAST>
 int launch_few(ApplyArgs a, cudaStream_t stream) {
     using S = ApplyShape<T, RP>;
-    a.k_split = split(a.tile_count, S::PER_SM, (a.d_in + S::K_CHUNK - 1) / S::K_CHUNK, MAX_K_SPLIT);
+    a.k_split = split(a.tile_count, S::PER_SM, (a.d_in + S::K_CHUNK - 1) / S::K_CHUNK, FEW_SHARES);
     a.col_split = split(a.tile_count, S::PER_SM, (a.d_out + S::COLUMNS - 1) / S::COLUMNS, 1 << 20);
     return launch_pair(adapter_down_kernel<T, RP, FAST>, adapter_up_kernel<T, RP, FAST>, a, S::SMEM1, S::SMEM2, stream);
 }
@@ -1085,7 +1089,7 @@ int launch_few(ApplyArgs a, cudaStream_t stream) {
 template <typename T, int RP, bool FAST>
 int launch_many(ApplyArgs a, cudaStream_t stream) {
     using S = TcShape<RP>;
-    a.k_split = split(a.tile_count, S::PER_SM1, (a.d_in + S::K_CHUNK - 1) / S::K_CHUNK, 4);   // every block of the second kernel adds the shares up
+    a.k_split = split(a.tile_count, S::PER_SM1, (a.d_in + S::K_CHUNK - 1) / S::K_CHUNK, MANY_SHARES);
     a.col_split = split(a.tile_count, S::PER_SM2, (a.d_out + S::COLUMNS - 1) / S::COLUMNS, 1 << 20);
     return launch_pair(adapter_down_tc_kernel<T, RP, FAST>, adapter_up_tc_kernel<T, RP, FAST>, a, S::SMEM1, S::SMEM2, stream);
 }
@@ -1113,10 +1117,14 @@ int grain_of(const void* p, long long stride_bytes) {
 
 int padded_rank(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
 
-// Shares of A x, at most MAX_K_SPLIT of them.
+// Shares of A x: of every tile one, or as many in all as blocks run at once (split).  Does not fall as batches grow, so the workspace of
+// the largest serves the others.
 size_t workspace_bytes(long long T, int n, int rank, int dtype) {
-    const int rows = takes_many(T, n, rank, dtype) ? MANY : FEW;
-    return sizeof(float) * MAX_K_SPLIT * (size_t)max_tiles(T, n, rows) * (size_t)rows * (size_t)padded_rank(rank);
+    const bool many = takes_many(T, n, rank, dtype);
+    const int rows = many ? MANY : FEW, rp = padded_rank(rank);
+    const long long tiles = max_tiles(T, n, rows), at_once = SMS * (many ? MANY_PER_SM : few_per_sm(rp));
+    const long long all = tiles * (many ? MANY_SHARES : FEW_SHARES), most = tiles > at_once ? tiles : at_once;
+    return sizeof(float) * (size_t)(all < most ? all : most) * (size_t)rows * (size_t)rp;
 }
 
 template <typename T>

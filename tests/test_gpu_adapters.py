@@ -517,3 +517,29 @@ def test_weights_whose_data_was_replaced():
         with pytest.raises(ValueError, match="must be a contiguous"):
             adapters.apply(x, y, plan)
         held[i].data = good
+
+
+@pytest.mark.parametrize("dtype,T,n,r,d", [("f32", 1, 1, 16, 2048), ("f32", 600, 3, 128, 512), ("f32", 9000, 2, 40, 64), ("bf16", 64, 64, 16, 2048),
+                                           ("bf16", 2048, 1, 64, 1024), ("f16", 4100, 3, 17, 512), ("bf16", 40000, 2, 64, 256)])
+def test_workspace_of_the_size_asked_for(dtype, T, n, r, d):
+    """A call writes nothing behind it, and its results are right with no byte more."""
+    import ctypes
+
+    from infmoe_b200 import capi
+    rng = np.random.default_rng(T)
+    t = TYPES[dtype]
+    x, y, a, b = whole(rng, (T, d), 2, t), whole(rng, (T, d), 50, t), whole(rng, (n, r, d), 2, t), whole(rng, (n, d, r), 1, t)
+    at = owners(rng, T, n, min(T, 9))
+    plan = Adapters(a, b).plan(torch.from_numpy(at).cuda())
+    code = {"f32": capi.DTYPE_F32, "f16": capi.DTYPE_F16, "bf16": capi.DTYPE_BF16}[dtype]
+    held, need = capi.AdapterSet(n, r, d, d, code, a.data_ptr(), b.data_ptr(), None, None), ctypes.c_size_t()
+    capi.check(capi.lib().infmoe_adapter_workspace_bytes(ctypes.byref(held), T, ctypes.byref(need)))
+    ws = torch.full((need.value + (16 << 20),), 77, dtype=torch.uint8, device="cuda")
+    out, status = torch.empty_like(y), torch.zeros(1, dtype=torch.int32, device="cuda")
+    capi.check(capi.lib().infmoe_adapter_apply(ctypes.byref(held), T, x.data_ptr(), d, y.data_ptr(), d, out.data_ptr(), d,
+                                               plan.buffer.data_ptr(), ws.data_ptr(), need.value, status.data_ptr(),
+                                               torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert int(status) == 0 and (ws[need.value:] == 77).all()
+    rows = np.unique(np.concatenate([np.arange(min(T, 300)), np.arange(max(0, T - 300), T)]))
+    check_exact(out[rows], reference(x[rows], y[rows], a, b, 1, None, at[rows]), t)

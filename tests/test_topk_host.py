@@ -196,3 +196,16 @@ def test_plans_of_more_rows_than_32_bits_count_are_refused(n):
         assert _apply(T=T, adapter_count=n, ws_bytes=1 << 60) == 6
         s = capi.AdapterSet(adapter_count=n, rank=8, d_in=32, d_out=48, dtype=2, d_a=SOME, d_b=SOME)
         assert lib.infmoe_adapter_workspace_bytes(ctypes.byref(s), T, ctypes.byref(need)) == 6
+
+
+def test_workspace_grows_with_what_a_call_uses():
+    """One share of A x for every place of the tiles in large batches, eight at most in small ones; enough for every smaller batch."""
+    lib, need = capi.lib(), ctypes.c_size_t()
+    for dtype, rank, padded, n in ((0, 128, 128, 8), (2, 128, 128, 8), (1, 33, 64, 3), (2, 16, 16, 64), (0, 20, 32, 1000), (1, 20, 32, 1)):
+        s = capi.AdapterSet(adapter_count=n, rank=rank, d_in=4096, d_out=4096, dtype=dtype, d_a=SOME, d_b=SOME)
+        before = 0
+        for T in sorted({1, 5, 16, 17, 100, 777, 2047, 2048, 4095, 4096, 32 * n - 1, 32 * n, 32 * n + 1, 131072, 1 << 20}):
+            assert lib.infmoe_adapter_workspace_bytes(ctypes.byref(s), T, ctypes.byref(need)) == 0
+            assert need.value >= max(before, 4 * padded * T)
+            before = need.value
+        assert need.value <= 4 * padded * (T + 128 * (n + 1))
