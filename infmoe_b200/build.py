@@ -21,6 +21,7 @@ OBJ = os.path.join(PKG, "build")
 LIB = os.path.join(PKG, "libinfmoe_b200.so")
 PLUGIN_LIB = os.path.join(PKG, "libtrtmoelayer.so")
 BINDING = os.path.join(PKG, "_binding.so")      # calls on torch tensors (csrc/binding.cc)
+BINDING_STAMP = os.path.join(OBJ, "_binding.made_for")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-fvisibility=hidden",
@@ -80,12 +81,26 @@ def _link(nvcc: str, objs, out: str, extra, verbose: bool) -> None:
             raise RuntimeError(f"link failed for {out}:\n{r.stdout}\n{r.stderr}")
 
 
+def _text(path: str) -> str:
+    try:
+        with open(path) as f:
+            return f.read()
+    except OSError:
+        return ""
+
+
 def _build_binding(verbose: bool) -> None:
-    """The extension module, compiled against the installed torch's headers."""
+    """The extension module, compiled against the installed torch's headers; compiled anew when torch or Python are other ones than
+    it was made for.  Without torch there is nothing to call it with, and the libraries alone are built."""
     src = os.path.join(CSRC, "binding.cc")
-    if not _stale(BINDING, [src, os.path.join(ROOT, "include", "infmoe_c.h")]):
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        print("torch is not installed: _binding.so is not built", file=sys.stderr)
         return
-    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
+    torch = spec.submodule_search_locations[0]
+    made_for = f"{sysconfig.get_config_var('SOABI')}\n{torch}\n" + _text(os.path.join(torch, "version.py"))
+    if not _stale(BINDING, [src, os.path.join(ROOT, "include", "infmoe_c.h")]) and _text(BINDING_STAMP) == made_for:
+        return
     cuda = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include")
     includes = [sysconfig.get_paths()["include"], os.path.join(torch, "include"),
                 os.path.join(torch, "include", "torch", "csrc", "api", "include"), cuda]
@@ -99,6 +114,8 @@ def _build_binding(verbose: bool) -> None:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for binding.cc:\n{r.stdout}\n{r.stderr}")
+    with open(BINDING_STAMP, "w") as f:
+        f.write(made_for)
 
 
 def build(verbose: bool = False) -> str:

@@ -209,3 +209,33 @@ def test_workspace_grows_with_what_a_call_uses():
             assert need.value >= max(before, 4 * padded * T)
             before = need.value
         assert need.value <= 4 * padded * (T + 128 * (n + 1))
+
+
+def test_binding_is_built_for_the_torch_that_is_there(monkeypatch, tmp_path):
+    import importlib.util
+    import subprocess
+
+    from infmoe_b200 import build
+
+    made = []
+
+    def compile_(cmd, **kw):
+        made.append(cmd)
+        with open(build.BINDING, "w") as f:
+            f.write("")
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(build, "BINDING", str(tmp_path / "_binding.so"))
+    monkeypatch.setattr(build, "BINDING_STAMP", str(tmp_path / "_binding.made_for"))
+    monkeypatch.setattr(build.subprocess, "run", compile_)
+    for _ in range(2):
+        build._build_binding(False)
+    assert len(made) == 1
+    text = build._text
+    monkeypatch.setattr(build, "_text", lambda path: "0.0" if path.endswith("version.py") else text(path))
+    for _ in range(2):
+        build._build_binding(False)
+    assert len(made) == 2
+    monkeypatch.setattr(importlib.util, "find_spec", lambda name: None)
+    build._build_binding(False)                                      # the libraries alone: no error
+    assert len(made) == 2
