@@ -239,3 +239,30 @@ def test_binding_is_built_for_the_torch_that_is_there(monkeypatch, tmp_path):
     monkeypatch.setattr(importlib.util, "find_spec", lambda name: None)
     build._build_binding(False)                                      # the libraries alone: no error
     assert len(made) == 2
+
+
+def _depth(body, at):
+    return body.count("{", 0, at) - body.count("}", 0, at)
+
+
+def _touches_results_behind_its_wait(body):
+    """The shares of A x and every store to memory come behind the one wait that is in no branch; in a branch, behind the branch's."""
+    waits = [m.start() for m in re.finditer(r"pdl_wait\(\)", body)]
+    main = [w for w in waits if _depth(body, w) == 1]
+    if len(main) != 1:
+        return False
+    uses = [m.start() for m in re.finditer(r"p\.sums|\*reinterpret_cast<uint4\*>\(out|\bdst\[|\bout_base\[|out_base \+", body)]
+    assert len(uses) >= 3 and "copy_rows<T>" in body
+    branch = body.rindex("{", 0, body.index("copy_rows<T>"))
+    return min(uses) > main[0] and any(branch < w < body.index("copy_rows<T>") for w in waits)
+
+
+@pytest.mark.parametrize("kernel", ["adapter_up_kernel", "adapter_up_tc_kernel"])
+def test_adapters_second_kernel_waits_for_the_first_ones_results(kernel):
+    with open(os.path.join(os.path.dirname(capi.LIB_PATH), "csrc", "adapters.cu")) as f:
+        body = _body(f.read(), kernel)
+    assert _touches_results_behind_its_wait(body)
+    waits = [m.start() for m in re.finditer(r"pdl_wait\(\);", body)]
+    assert len(waits) == 3                       # an empty tile's, a tile's without adapter, the others'
+    for w in waits[1:]:
+        assert not _touches_results_behind_its_wait(body[:w] + body[w + len("pdl_wait();"):])
