@@ -230,6 +230,49 @@ def test_select_refuses_a_bias_that_was_replaced():
             router.select(l)
 
 
+def choice_of_all(l, k, score, bias, groups, top_groups, group_best, renormalise):
+    """topk_ref.select for many rows at once, in 64 bits on the GPU."""
+    T, E = l.shape
+    ok = l > torch.finfo(l.dtype).min
+    d = torch.where(ok, l.double(), -torch.inf)
+    p = torch.softmax(d, 1).nan_to_num(0) if score == "softmax" else torch.where(ok, torch.sigmoid(d), 0.0)
+    c = torch.where(ok, p + bias.double(), -torch.inf) if bias is not None else d
+    if groups > 1:
+        best = torch.where(ok, c if bias is not None or group_best == 1 else p, -torch.inf).view(T, groups, -1).topk(min(2, E // groups), 2).values
+        value = best[:, :, 0]
+        if group_best == 2 and best.shape[2] == 2:
+            value = value + torch.where(best[:, :, 1] > -torch.inf, best[:, :, 1], 0.0)
+        order = value.sort(dim=1, descending=True, stable=True).indices
+        out = torch.zeros(T, groups, dtype=torch.bool, device="cuda").scatter(1, order[:, top_groups:], True)
+        c = c.masked_fill(out.repeat_interleave(E // groups, 1), -torch.inf)
+    value, gate = c.sort(dim=1, descending=True, stable=True)
+    gate, none = gate[:, :k], value[:, :k] == -torch.inf
+    w = p.gather(1, gate).masked_fill(none, 0.0)
+    if renormalise:
+        w = (w / w.sum(1, keepdim=True)).nan_to_num(0)
+    return gate.masked_fill(none, -1).to(torch.int32), w
+
+
+@pytest.mark.parametrize("dtype,score,E,k,groups,top_groups,group_best,bias,renormalise", [
+    ("f32", "softmax", 24, 4, 1, 1, 1, False, True), ("bf16", "softmax", 64, 2, 1, 1, 1, False, False),
+    ("f16", "sigmoid", 120, 6, 5, 3, 2, True, True), ("f32", "sigmoid", 256, 8, 8, 4, 2, True, True),
+    ("f32", "softmax", 256, 20, 8, 4, 1, False, True), ("bf16", "softmax", 512, 16, 1, 1, 1, True, False),
+    ("f32", "sigmoid", 1000, 7, 1, 1, 1, True, True)])
+@pytest.mark.parametrize("T", [10000, 160000])
+def test_select_of_many_tokens(T, dtype, score, E, k, groups, top_groups, group_best, bias, renormalise):
+    """A warp's second token comes after 2368 to 4736 of them, a block's second 32 turns after 75776 to 151552."""
+    l = logits_of(T, E, TYPES[dtype], E)
+    l[::97] = -torch.inf
+    l[1::101, E // 2:] = torch.nan
+    b = torch.from_numpy(np.random.default_rng(E).standard_normal(E).astype(np.float32) * 0.1).cuda() if bias else None
+    router = TopKRouter(E, k, score=score, bias=b, groups=groups, top_groups=top_groups, group_best=group_best, renormalise=renormalise)
+    gate, weight = router.select(l)
+    for t0 in range(0, T, 20000):
+        want, w = choice_of_all(l[t0:t0 + 20000], k, score, b, groups, top_groups, group_best, renormalise)
+        assert torch.equal(gate[t0:t0 + 20000], want)
+        torch.testing.assert_close(weight[t0:t0 + 20000].double(), w, rtol=WEIGHT_TOL, atol=1e-37)
+
+
 def slots_of(T, k, E, none=0.1, seed=0):
     rng = np.random.default_rng(seed)
     gate = np.stack([rng.permutation(E)[:k] for _ in range(T)]).astype(np.int32) if T else np.zeros((0, k), np.int32)
@@ -264,6 +307,26 @@ def test_rows_to_their_experts_and_back(T, k, D, E, dtype):
     for residual in (None, x):
         got = combine_topk(y, weight, row_of=row_of, residual=residual)
         check_combined(got, y, weight, row_of.cpu().numpy(), residual)
+
+
+@pytest.mark.parametrize("dtype,T,k,D", [("f32", 700, 4, 1024), ("f32", 3000, 3, 1001), ("bf16", 3000, 3, 1001), ("f16", 2500, 2, 1002),
+                                         ("bf16", 300001, 3, 5), ("f32", 250000, 3, 3), ("f16", 150000, 8, 8), ("f32", 5, 2, 300004)])
+def test_many_rows_to_their_experts(dtype, T, k, D):
+    """More than 8 MB of them: four rows to a thread, by 16, 4 and 2 bytes, long rows and short ones."""
+    t, E = TYPES[dtype], 60
+    g = torch.Generator(device="cuda").manual_seed(T)
+    x = torch.randn(T, D, device="cuda", generator=g).to(t)
+    gate = torch.randint(0, E, (T, k), device="cuda", generator=g, dtype=torch.int32)
+    gate[torch.rand(T, device="cuda", generator=g) < 0.1] = -1
+    pos, _, offset = count_experts(gate, E)
+    routed, row_of = scatter_topk(x, pos, offset, k, out=torch.full((T * k, D), 7.0, device="cuda", dtype=t))
+    flat = gate.flatten().long()
+    order = torch.where(flat < 0, E, flat).sort(stable=True).indices
+    n = int((flat >= 0).sum())
+    want_row = torch.full((T * k,), -1, dtype=torch.int32, device="cuda")
+    want_row[order[:n]] = torch.arange(n, dtype=torch.int32, device="cuda")
+    assert int(offset[-1]) == n and torch.equal(row_of.flatten(), want_row)
+    assert torch.equal(routed[:n], x[order[:n] // k]) and (routed[n:] == 7).all()
 
 
 def check_combined(got, y, weight, row_of, residual):
