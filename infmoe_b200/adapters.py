@@ -12,6 +12,7 @@ from __future__ import annotations
 import ctypes
 
 from . import capi
+from .plugin import _current_stream
 from .topk import binding, check_array, launch
 
 __all__ = ["Adapters", "AdapterPlan"]
@@ -29,6 +30,7 @@ class AdapterPlan:
         need = ctypes.c_size_t()
         capi.check(capi.lib().infmoe_adapter_plan_bytes(self.tokens, self.adapter_count, ctypes.byref(need)))
         self.buffer = torch.empty(need.value, dtype=torch.uint8, device=self.device)
+        self._home = _current_stream(torch, adapter_of_token.get_device())      # that the buffer was allocated on
         launch(adapter_of_token.get_device(), "infmoe_adapter_plan", self.tokens, self.adapter_count,
                adapter_of_token.data_ptr(), self.buffer.data_ptr(), need.value)
 
@@ -49,8 +51,13 @@ class Adapters:
         n, r, d_in = a.shape
         self.dtype, self.device = a.dtype, a.device
         self.adapter_count, self.rank, self.d_in, self.d_out = n, r, d_in, b.shape[1]
+        self._home = None                            # the stream that a scale made here was allocated on
         if isinstance(scale, (int, float)):
-            scale = None if scale == 1 else torch.full((n,), float(scale), dtype=torch.float32, device=a.device)
+            if scale == 1:
+                scale = None
+            else:
+                scale = torch.full((n,), float(scale), dtype=torch.float32, device=a.device)
+                self._home = _current_stream(torch, a.get_device())
         if scale is not None:
             check_array(scale, (n,), torch.float32, a.device, "scale")
         if rank is not None:
@@ -73,4 +80,5 @@ class Adapters:
         """x [..., d_in], y [..., d_out] -> y plus each row's adapter of x.  out may be y (in place), not x.
 
         status (int32 [1], may be None): bit 2 is set when a bounded wait inside a kernel ran out."""
-        return self._apply(self._set, *self._tensors, x, y, plan.buffer, plan.tokens, plan.adapter_count, out, status)
+        return self._apply(self._set, *self._tensors, x, y, plan.buffer, plan.tokens, plan.adapter_count, out, status, self._home,
+                           plan._home)

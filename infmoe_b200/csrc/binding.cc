@@ -100,8 +100,17 @@ void* data(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // Device and torch's current stream for the call.
 struct On {
-    explicit On(const at::Tensor& t) : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()) {}
+    explicit On(const at::Tensor& t) : guard(t.device()), current(c10::cuda::getCurrentCUDAStream(t.device().index())), stream(current.stream()) {}
+    // Memory that a plan or a set allocated itself, on stream `home` (a handle; None: it is the caller's), is not given to others of that
+    // stream before this one is done with it.
+    void uses(const at::Tensor& t, PyObject* home) const {
+        if (home == Py_None) return;
+        void* const h = PyLong_AsVoidPtr(home);
+        if (!h && PyErr_Occurred()) throw Refused{};
+        if (h != stream) t.record_stream(current.unwrap());
+    }
     c10::cuda::CUDAGuard guard;
+    c10::cuda::CUDAStream current;
     void* stream;
 };
 
@@ -217,8 +226,8 @@ PyObject* combine_topk(PyObject* const* a) {
     return wrap(out);
 }
 
-// (bytes of the set, a, b, scale, rank, x, y, plan buffer, plan tokens, plan adapters, out, status) -> out.  Where the weights lie is asked of the
-// tensors at every call: a parameter's data may have been replaced since the set was made.
+// (bytes of the set, a, b, scale, rank, x, y, plan buffer, plan tokens, plan adapters, out, status, scale's stream, plan's stream) -> out.  Where
+// the weights lie is asked of the tensors at every call: a parameter's data may have been replaced since the set was made.
 PyObject* apply_adapters(PyObject* const* args) {
     if (!PyBytes_Check(args[0]) || PyBytes_GET_SIZE(args[0]) != (Py_ssize_t)sizeof(infmoe_adapter_set)) refuse("not an adapter set");
     infmoe_adapter_set set;
@@ -261,6 +270,8 @@ PyObject* apply_adapters(PyObject* const* args) {
     const at::Tensor workspace = at::detail::empty_cuda({(int64_t)bytes}, at::kByte, device, std::nullopt);
     check(infmoe_adapter_apply(&set, rx.count, x.data_ptr(), rx.ld, y.data_ptr(), ry.ld, out.data_ptr(), ldo, plan.data_ptr(),
                                workspace.data_ptr(), bytes, (int32_t*)data(status), on.stream));
+    if (scale) on.uses(*scale, args[12]);
+    on.uses(plan, args[13]);
     return wrap(out);
 }
 
@@ -268,7 +279,7 @@ PyMethodDef methods[] = {
     {"select_topk", (PyCFunction)(void (*)())Entry<select_topk>::call<6>, METH_FASTCALL, nullptr},
     {"scatter_topk", (PyCFunction)(void (*)())Entry<scatter_topk>::call<6>, METH_FASTCALL, nullptr},
     {"combine_topk", (PyCFunction)(void (*)())Entry<combine_topk>::call<6>, METH_FASTCALL, nullptr},
-    {"apply_adapters", (PyCFunction)(void (*)())Entry<apply_adapters>::call<12>, METH_FASTCALL, nullptr},
+    {"apply_adapters", (PyCFunction)(void (*)())Entry<apply_adapters>::call<14>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -543,3 +543,29 @@ def test_workspace_of_the_size_asked_for(dtype, T, n, r, d):
     assert int(status) == 0 and (ws[need.value:] == 77).all()
     rows = np.unique(np.concatenate([np.arange(min(T, 300)), np.arange(max(0, T - 300), T)]))
     check_exact(out[rows], reference(x[rows], y[rows], a, b, 1, None, at[rows]), t)
+
+
+def test_plan_given_up_while_another_stream_still_needs_it():
+    """What a plan and a set allocate themselves stays theirs until the calls on other streams that read it are done."""
+    rng = np.random.default_rng(43)
+    n, r, d, T = 3, 8, 64, 500
+    x, y, a, b = whole(rng, (T, d), 2, torch.float32), whole(rng, (T, d), 9, torch.float32), whole(rng, (n, r, d), 2, torch.float32), \
+        whole(rng, (n, d, r), 1, torch.float32)
+    at = owners(rng, T, n, 7)
+    dat = torch.from_numpy(at).cuda()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            adapters = Adapters(a, b, scale=0.5)
+            plan = adapters.plan(dat)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda._sleep(40_000_000)                               # about 20 ms
+        got = adapters.apply(x, y, plan)
+        size = plan.buffer.numel()
+        del plan, adapters
+        with torch.cuda.stream(side):                               # zeros: a plan of no rows, a scale of zero
+            taken = [torch.zeros(size, dtype=torch.uint8, device="cuda"), torch.zeros(n, device="cuda")]
+        side.synchronize()
+        check_exact(got, reference(x, y, a, b, 0.5, None, at), torch.float32)
+        del taken
