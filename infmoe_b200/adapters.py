@@ -56,7 +56,9 @@ class Adapters:
             if scale == 1:
                 scale = None
             else:
-                scale = torch.full((n,), float(scale), dtype=torch.float32, device=a.device)
+                # copied from the host, so that it is there for calls on any stream (a capture cannot wait for that)
+                at = a.device if torch.cuda.is_current_stream_capturing() else "cpu"
+                scale = torch.full((n,), float(scale), dtype=torch.float32, device=at).to(a.device)
                 self._home = _current_stream(torch, a.get_device())
         if scale is not None:
             check_array(scale, (n,), torch.float32, a.device, "scale")

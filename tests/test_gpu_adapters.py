@@ -569,3 +569,26 @@ def test_plan_given_up_while_another_stream_still_needs_it():
         side.synchronize()
         check_exact(got, reference(x, y, a, b, 0.5, None, at), torch.float32)
         del taken
+
+
+def test_scale_is_there_when_the_set_is():
+    """A number for a scale becomes a tensor on the device, of which other streams know nothing."""
+    rng = np.random.default_rng(47)
+    r, d, T = 8, 64, 64
+    x, y = whole(rng, (T, d), 2, torch.float32), whole(rng, (T, d), 9, torch.float32)
+    a, b = whole(rng, (3, r, d), 2, torch.float32), whole(rng, (3, d, r), 1, torch.float32)
+    at = owners(rng, T, 3, 7)
+    plan = AdapterPlan(torch.from_numpy(at).cuda(), 3)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for scale in (0.5, 0.25, 4.0):
+        before = torch.full((3,), 3.0, device="cuda")
+        torch.cuda.synchronize()
+        del before                                                  # its memory is the next scale's
+        torch.cuda._sleep(40_000_000)
+        adapters = Adapters(a, b, scale=scale)
+        with torch.cuda.stream(side):
+            got = adapters.apply(x, y, plan)
+        side.synchronize()
+        check_exact(got, reference(x, y, a, b, scale, None, at), torch.float32)
+        torch.cuda.synchronize()
