@@ -152,7 +152,9 @@ INFMOE_API int infmoe_layer_expert_forward_scatter(infmoe_layer* layer, const fl
  * d_weight [token_num][top_k] come from infmoe_expert_select_topk; a gate outside [0, expert_count) is a place without an
  * expert, and a token without any passes unchanged.  Experts resident, streamed or of a registered sublayer as in
  * infmoe_layer_enqueue; the variant's own routing and output mix play no part, and
- * infmoe_layer_last_routing stays that of the last enqueue.  No counterpart in the reference (top-1). */
+ * infmoe_layer_last_routing stays that of the last enqueue.  Refused (INFMOE_ERR_UNSUPPORTED) where token_num * top_k *
+ * max(embedding_size, hidden_size) exceeds 2^31 - 1, infmoe_layer_enqueue's own limit for that many rows.  No counterpart in the
+ * reference (top-1). */
 INFMOE_API int infmoe_layer_topk_workspace_bytes(const infmoe_layer* layer, int64_t token_num, int32_t top_k, size_t* bytes);
 INFMOE_API int infmoe_layer_forward_topk(infmoe_layer* layer, const float* d_input, const int32_t* d_gate,
                                          const float* d_weight, int64_t token_num, int32_t top_k, float* d_output,
@@ -414,7 +416,9 @@ INFMOE_API int infmoe_t5ff_run_static(int64_t rows, int32_t embedding_size, int3
 /* No counterparts in the reference (top-k routing is a TODO there).  Unlike the
  * functions above these take FP32, FP16 or BF16 elements; all of them compute in
  * FP32 or more and round once, when they store.  FP32 adapters form a product from
- * two parts of 11 bits to each factor: off by at most 2^-21 of it, to either side. */
+ * two parts of 11 bits to each factor: off by at most 2^-21 of it, to either side.
+ * 16-bit adapters hold A x as two parts of the type (16 bits and more), and an
+ * infinity in B may then come out as NaN. */
 typedef enum infmoe_dtype { INFMOE_F32 = 0, INFMOE_F16 = 1, INFMOE_BF16 = 2 } infmoe_dtype;
 typedef enum infmoe_score { INFMOE_SCORE_SOFTMAX = 0, INFMOE_SCORE_SIGMOID = 1 } infmoe_score;
 
@@ -433,7 +437,8 @@ typedef struct infmoe_topk_config {
  * elements, >= expert_count): gating logits.  Scores s are the softmax of a row or the sigmoid of each logit; experts and
  * groups are chosen by s + d_bias[e] (d_bias [expert_count] or NULL: none), weights are s alone, so a bias balances the load
  * without showing in the result.  The choice is that of these sums in 64 bits (without a bias experts stand in the order of
- * their logits, and so do groups that count with one expert); ties go to the lowest index.
+ * their logits, and so do groups that count with one expert); ties go to the lowest index, +0 and -0 being one value.  More
+ * than 16 experts to a token cost several times what 16 do: 32 bits no longer help with the choice.
  * An expert whose logit is NaN or the type's lowest value or less (-inf included) is never chosen and is no part of the
  * softmax; one whose bias is NaN or -inf is never chosen.  Where fewer than top_k experts are left, the remaining places get
  * gate -1 and weight 0; a token with none at all also sets bit 0 of d_status (may be NULL), like infmoe_expert_select.

@@ -81,6 +81,8 @@ class Adapters:
     def apply(self, x, y, plan: AdapterPlan, out=None, status=None):
         """x [..., d_in], y [..., d_out] -> y plus each row's adapter of x.  out may be y (in place), not x.
 
-        status (int32 [1], may be None): bit 2 is set when a bounded wait inside a kernel ran out."""
+        status (int32 [1], may be None): bit 2 is set when a bounded wait inside a kernel ran out.  The result is then not complete,
+        and without a status nothing says so.  A plan may be used, and given up, on other streams than that it was made on, once
+        they have waited for it."""
         return self._apply(self._set, *self._tensors, x, y, plan.buffer, plan.tokens, plan.adapter_count, out, status, self._home,
                            plan._home)

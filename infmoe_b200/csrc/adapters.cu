@@ -6,7 +6,7 @@
 // y + scale B v, which starts under the first and fetches y and B meanwhile.  A token costs 2 r (d_in + d_out) products for its
 // (d_in + 2 d_out) elements, so memory bounds large batches and the latency of two kernels small ones.  Device time and what
 // the bytes take at the copy rate, us: 64 tokens and as many adapters of rank 16, 4096 x 4096, BF16 7.5 and 1.9; 4096 tokens, 8 of
-// rank 16 21.8 and 15.3; 777 tokens of up to rank 24, 1000 x 2724, FP32 14.3 and 3.2; 16384 tokens of rank 64, 4096 x 10240, FP16
+// rank 16 21.9 and 15.3; 777 tokens of up to rank 24, 1000 x 2724, FP32 13.9 and 3.2; 16384 tokens of rank 64, 4096 x 10240, FP16
 // 182 and 129.  As one kernel, with clusters and distributed shared memory, the second of these took 25.3.
 #include <cfloat>
 #include <climits>
@@ -1104,7 +1104,8 @@ int launch_apply_rank(const ApplyArgs& a, bool many, bool fast, cudaStream_t str
 // Tiles of MANY rows or of FEW.  In 16 bits, with many tokens to an adapter, the wide ranks keep mma.sync busier than the memory.
 // Measured, FEW and MANY, us, 4096 x 4096 in BF16: rank 16, 16384 tokens 74 and 89; rank 32, 2048 tokens 18 and 26, 4096 tokens
 // 36 and 34, 16384 tokens 105 and 91; rank 64, 1024 tokens 21 and 22, 2048 tokens 32 and 30, 4096 tokens 43 and 39.  FP32 has
-// three TF32 products to each and stays with FEW.
+// three TF32 products to each and stays with FEW.  These lines hold for all widths and go by the adapters that are loaded, not by those that a
+// batch uses: 16384 tokens of rank 64 with 1000 loaded and one used stay with FEW.
 bool takes_many(long long T, int n, int rank, int dtype) {
     return dtype != INFMOE_F32 && T >= 32ll * n && rank > 16 && T >= (rank > 32 ? 2048 : 4096);
 }

@@ -330,7 +330,7 @@ class MoELayer:
         [0, expert_count): none) with the weights weight [..., k] (float32): x + sum_s weight_s (E_s(x) - x).
 
         gate and weight are what TopKRouter.select returns.  On torch's current stream; the workspace comes from torch's
-        allocator and goes back to it."""
+        allocator and goes back to it.  Tokens times k times the larger of d_model and d_ff must stay below 2^31."""
         import torch
 
         from .topk import check_array, launch

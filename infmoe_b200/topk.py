@@ -89,7 +89,9 @@ class TopKRouter:
         """logits: float32, float16 or bfloat16 CUDA tensor [..., expert_count] -> (gate int32, weight float32), [..., top_k].
 
         Experts with a logit of NaN or of the type's lowest value or less (-inf) are not chosen; places that stay empty hold
-        gate -1 and weight 0.  status (int32 [1], may be None): bit 0 is set when a token has no expert at all."""
+        gate -1 and weight 0.  More than 16 experts to a token cost several times what 16 do.
+
+        status (int32 [1], may be None): bit 0 is set when a token has no expert at all."""
         return self._select(self._cfg, logits, self.bias, gate, weight, status)
 
 
