@@ -592,3 +592,27 @@ def test_scale_is_there_when_the_set_is():
         side.synchronize()
         check_exact(got, reference(x, y, a, b, scale, None, at), torch.float32)
         torch.cuda.synchronize()
+
+
+def test_captured_with_a_plan_made_before():
+    """The stream of a capture is another one than the plan's; a set may be made within it."""
+    rng = np.random.default_rng(53)
+    T, n, r, d = 90, 3, 8, 64
+    x, y, a, b = whole(rng, (T, d), 2, torch.float32), whole(rng, (T, d), 9, torch.float32), whole(rng, (n, r, d), 2, torch.float32), \
+        whole(rng, (n, d, r), 1, torch.float32)
+    at = owners(rng, T, n, 5)
+    first = Adapters(a, b, scale=0.5)
+    plan = first.plan(torch.from_numpy(at).cuda())
+    first.apply(x, y, plan)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        second = Adapters(a, b, scale=2.0)
+        out = second.apply(x, first.apply(x, y, plan), plan)
+    for _ in range(2):
+        x.copy_(whole(rng, (T, d), 2, torch.float32))
+        g.replay()
+        torch.cuda.synchronize()
+        check_exact(out, reference(x, y, a, b, 2.5, None, at), torch.float32)
+    del g, first, second, plan
+    assert torch.equal(torch.zeros(4096, device="cuda"), torch.zeros(4096, device="cuda"))   # the allocator's work goes on
